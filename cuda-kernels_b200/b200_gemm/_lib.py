@@ -20,6 +20,7 @@ B200_ERR_TENSOR_MAP = 5
 B200_ERR_DEVICE_TIMEOUT = 6
 B200_ERR_TOO_LARGE = 7
 B200_ERR_SCRATCH_LIMIT = 8
+B200_ERR_BAD_INDEX = 9
 
 B200_B_NK = 0
 B200_B_KN = 1
@@ -44,6 +45,22 @@ class Epilogue(ctypes.Structure):
     _fields_ = [("alpha", ctypes.c_float), ("beta", ctypes.c_float), ("c_in", ctypes.c_void_p),
                 ("ldc_in", ctypes.c_int64), ("bias", ctypes.c_void_p), ("d_dtype", ctypes.c_int)]
 
+
+class AttnView(ctypes.Structure):
+    """b200_attn_view (include/b200_gemm.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("seq_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class KvCache(ctypes.Structure):
+    """b200_kv_cache (include/b200_gemm.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int64)]
+
+
+_VIEW = ctypes.POINTER(AttnView)
+_CACHE = ctypes.POINTER(KvCache)
 
 # Every symbol include/b200_gemm.h declares, with its ctypes signature.
 _SIGNATURES = {
@@ -94,6 +111,18 @@ _SIGNATURES = {
     "b200_flash_attn_bf16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                             ctypes.c_int64, ctypes.c_int, ctypes.c_void_p]),
+    "b200_kv_cache_write": (ctypes.c_int, [_VIEW, _VIEW, _CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                           ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
+    "b200_cache_attn_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _CACHE,
+                                                       ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_cache_attn": (ctypes.c_int, [_VIEW, _CACHE, ctypes.c_void_p, ctypes.c_void_p, _VIEW, ctypes.c_int64,
+                                       ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p,
+                                       ctypes.c_size_t, ctypes.c_void_p]),
+    "b200_cross_attn_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                                       ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_cross_attn_bf16": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, ctypes.c_void_p, _VIEW, ctypes.c_void_p, ctypes.c_int64,
+                                            ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                            ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "b200_gemm_bf16_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                               ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                               ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,

@@ -49,6 +49,7 @@ def _nvcc() -> str:
 
 def _sources() -> list[str]:
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
+                  + glob.glob(os.path.join(CSRC, "*.h"))
                   + [os.path.join(INCLUDE, "b200_gemm.h")])
 
 
@@ -65,7 +66,7 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     cus = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     tmp = LIB_PATH + ".tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-I", INCLUDE, "-o", tmp, *cus]
+    cmd = [_nvcc(), *NVCC_FLAGS, "--threads", "0", "-shared", "-I", INCLUDE, "-o", tmp, *cus]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), flush=True)

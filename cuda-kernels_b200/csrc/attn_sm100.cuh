@@ -36,6 +36,16 @@
 // tile's MMAs); poly_exp2x2 can move a share of them to the FMA pipe
 // (kAttnPolyEvery).
 // Every wait is bounded (status bits on expiry), as in the GEMM kernels.
+//
+// flash_attn_fwd_kernel<true> is cross attention (b200_cross_attn_bf16): keys
+// of another length than the queries, a device array of key lengths (one per
+// batch entry), strided operands (4-D tensor maps), and the log-sum-exp of
+// every row for the backward pass.  Its pipeline is the one above with a full
+// mask.  What differs: the key count is read on the device; scores of keys at
+// or past it are -inf; their V rows may hold anything (NaN included), and
+// 0 x NaN would reach O through the product, so the two idle warps zero those
+// rows of the last V tile in shared memory before its product; a batch entry
+// without keys writes O = 0 and lse = -inf.
 #pragma once
 
 #include <cuda.h>
@@ -96,6 +106,10 @@ struct AttnParams {
   float scale_log2;  // log2(e) / sqrt(D): scores go straight to the exp2 domain
   uint64_t timeout_ns;
   uint32_t* status;
+  // Cross attention only.
+  int32_t kv_len;          // rows of K and V
+  const int32_t* kv_lens;  // [batch] keys of each batch entry (clamped to [0, kv_len]), or NULL: kv_len
+  float* lse;              // [batch, heads, seq_len] natural log of the softmax denominator, or NULL
 };
 
 struct AttnSmemPlan {
@@ -106,7 +120,7 @@ struct AttnSmemPlan {
   static constexpr int kOffBar = kOffV + kAttnVStages * kTileBytes;
   // q_full[Q], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[Q], p_full[Q][2], o_full[Q], drain
   static constexpr int kRingBars = kAttnQTiles + 2 * kAttnKStages + 2 * kAttnVStages;
-  static constexpr int kNumBars = kRingBars + 4 * kAttnQTiles + 1;
+  static constexpr int kNumBars = kRingBars + 4 * kAttnQTiles + 2;  // + v_raw (cross attention)
   static constexpr int kOffTmemHolder = kOffBar + kNumBars * 8;
   static constexpr int kOffAbort = kOffTmemHolder + 4;
   static constexpr int kBytes = kOffAbort + 4;
@@ -181,14 +195,21 @@ __device__ __forceinline__ float row_exp(const float* x, float scale, float m_us
   return s.x + s.y;
 }
 
-__device__ __forceinline__ void attn_raise(const AttnParams& p, volatile uint32_t* abort_flag, uint32_t code) {
+template <typename Params>
+__device__ __forceinline__ void attn_raise(const Params& p, volatile uint32_t* abort_flag, uint32_t code) {
   *abort_flag = 1u;
   if (p.status != nullptr) atomicOr(p.status, code);
+}
+
+// Keys of batch entry `bat` in cross attention.
+__device__ __forceinline__ int attn_kv_len(const int32_t* kv_lens, int bat, int kv_len) {
+  return kv_lens != nullptr ? min(max(kv_lens[bat], 0), kv_len) : kv_len;
 }
 
 // Grid (heads * batch, ceil(num_q_tiles / 2)).  Blocks start in linear
 // order, x fastest, and query tile pairs are taken in reverse order of y: the
 // longest causal rows of every head start first (longest-first scheduling).
+template <bool kCross>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     flash_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                           const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -215,6 +236,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto p_full = [&](int i, int h) { return bar0 + 8u * (Plan::kRingBars + kAttnQTiles + 2 * i + h); };
   auto o_full = [&](int i) { return bar0 + 8u * (Plan::kRingBars + 3 * kAttnQTiles + i); };
   const uint32_t drain = bar0 + 8u * (Plan::kRingBars + 4 * kAttnQTiles);  // every MMA issued has completed
+  const uint32_t v_raw = drain + 8u;  // cross attention: the last V tile has landed, its rows past the last key not yet zero
   // Ring slot and phase parity of key tile j.
   auto k_slot = [](int j) { return j % kAttnKStages; };
   auto k_par = [](int j) { return (uint32_t)(j / kAttnKStages) & 1u; };
@@ -237,18 +259,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
   const int head = (int)blockIdx.x % p.heads;
   const int bat = (int)blockIdx.x / p.heads;
-  const int kv_tiles_all = (p.seq_len + kAttnBKV - 1) / kAttnBKV;
-  // Key tiles query tile qt reads (the causal mask ends at the diagonal tile);
-  // 0 for a second tile past the end of the sequence.
-  auto kv_tiles = [&](int qt) {
-    return qt >= p.num_q_tiles ? 0 : (p.causal ? min(qt + 1, kv_tiles_all) : kv_tiles_all);
-  };
-  const int n0 = kv_tiles(qt_of[0]);
-  const int n1 = kv_tiles(qt_of[1]);  // >= n0, or 0
-  const int n_max = max(n0, n1);
-  const int n_q = n1 > 0 ? 2 : 1;    // query tiles this CTA holds
   const int col0 = head * kAttnD;                  // column of this head in the [seq, heads * D] view
-  const int kv_col0 = (head / p.group) * kAttnD;   // its key/value head in [seq, kv_heads * D]
+  const int kv_head = head / p.group;
+  const int kv_col0 = kv_head * kAttnD;            // its key/value head in [seq, kv_heads * D]
 
   if (warp == kAttnProducerWarp && lane == 0) {
     for (int i = 0; i < kAttnQTiles; ++i) {
@@ -267,6 +280,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(v_empty(s), 1);
     }
     mbar_init(drain, 1);
+    if constexpr (kCross) mbar_init(v_raw, 1);
     *abort_flag = 0u;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -284,6 +298,20 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t tmem_base = *tmem_holder;  // S_i at columns 128 i, O_i at 256 + 128 i
   pdl_launch_dependents();
   pdl_wait();
+  int kv_len = p.seq_len;  // keys of this batch entry (device data in cross attention: after the launch wait)
+  if constexpr (kCross) kv_len = attn_kv_len(p.kv_lens, bat, p.kv_len);
+  const int kv_tiles_all = (kv_len + kAttnBKV - 1) / kAttnBKV;
+  // Key tiles query tile qt reads (the causal mask ends at the diagonal tile);
+  // 0 for a second tile past the end of the sequence.
+  auto kv_tiles = [&](int qt) {
+    return qt >= p.num_q_tiles ? 0 : (p.causal ? min(qt + 1, kv_tiles_all) : kv_tiles_all);
+  };
+  const int n0 = kv_tiles(qt_of[0]);
+  const int n1 = kv_tiles(qt_of[1]);  // >= n0, or 0
+  const int n_max = max(n0, n1);
+  const int n_q = n1 > 0 ? 2 : (n0 > 0 ? 1 : 0);  // query tiles this CTA reads
+  // Rows of the last V tile past the last key, which TMA filled from memory.
+  const bool clean_v = kCross && kv_len < p.kv_len && kv_len % kAttnBKV != 0;
 
   if (warp >= kAttnProducerWarp) {
     setmaxnreg_dec<kAttnRegsOther>();
@@ -295,8 +323,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int i = 0; i < n_q; ++i) {
           mbar_arrive_expect_tx(q_full(i), Plan::kTileBytes);
           for (int h = 0; h < 2; ++h) {
-            tma_load_3d(sQ + i * Plan::kTileBytes + h * 16384, &tmQ, q_full(i), col0 + 64 * h,
-                        qt_of[i] * kAttnBQ, bat, pol_once);
+            if constexpr (kCross) {
+              tma_load_4d(sQ + i * Plan::kTileBytes + h * 16384, &tmQ, q_full(i), 64 * h, head, qt_of[i] * kAttnBQ, bat,
+                          pol_once);
+            } else {
+              tma_load_3d(sQ + i * Plan::kTileBytes + h * 16384, &tmQ, q_full(i), col0 + 64 * h,
+                          qt_of[i] * kAttnBQ, bat, pol_once);
+            }
           }
         }
         bool ok = true;
@@ -309,20 +342,33 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
           mbar_arrive_expect_tx(k_full(sk), Plan::kTileBytes);
           for (int h = 0; h < 2; ++h) {
-            tma_load_3d(sK + sk * Plan::kTileBytes + h * 16384, &tmK, k_full(sk), kv_col0 + 64 * h, j * kAttnBKV,
-                        bat, pol_keep);
+            if constexpr (kCross) {
+              tma_load_4d(sK + sk * Plan::kTileBytes + h * 16384, &tmK, k_full(sk), 64 * h, kv_head, j * kAttnBKV, bat,
+                          pol_keep);
+            } else {
+              tma_load_3d(sK + sk * Plan::kTileBytes + h * 16384, &tmK, k_full(sk), kv_col0 + 64 * h, j * kAttnBKV,
+                          bat, pol_keep);
+            }
           }
           ++k_issued;
           if (!mbar_wait(v_empty(sv), v_par(j) ^ 1u, p.timeout_ns, abort_flag)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(v_full(sv), Plan::kTileBytes);
+          // A tile to be cleaned lands on a barrier of its own; v_full then
+          // comes from the cleaning warps (which, outside the ring, could
+          // miss a phase of v_full).
+          const uint32_t v_bar = clean_v && j == n_max - 1 ? v_raw : v_full(sv);
+          mbar_arrive_expect_tx(v_bar, Plan::kTileBytes);
           // V tile as two 64-key halves, each two 64-column atoms of [64 keys][64 d].
           for (int hk = 0; hk < 2; ++hk) {
             for (int h = 0; h < 2; ++h) {
-              tma_load_3d(sV + sv * Plan::kTileBytes + hk * 16384 + h * 8192, &tmV, v_full(sv), kv_col0 + 64 * h,
-                          j * kAttnBKV + 64 * hk, bat, pol_keep);
+              const uint32_t dst = sV + sv * Plan::kTileBytes + hk * 16384 + h * 8192;
+              if constexpr (kCross) {
+                tma_load_4d(dst, &tmV, v_bar, 64 * h, kv_head, j * kAttnBKV + 64 * hk, bat, pol_keep);
+              } else {
+                tma_load_3d(dst, &tmV, v_bar, kv_col0 + 64 * h, j * kAttnBKV + 64 * hk, bat, pol_keep);
+              }
             }
           }
           ++v_issued;
@@ -335,7 +381,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           drained = mbar_wait(k_full(k_slot(j)), k_par(j), p.timeout_ns, nullptr);
         }
         for (int j = v_issued - 1; drained && j >= 0 && j >= v_issued - kAttnVStages; --j) {
-          drained = mbar_wait(v_full(v_slot(j)), v_par(j), p.timeout_ns, nullptr);
+          drained = clean_v && j == n_max - 1 ? mbar_wait(v_raw, 0u, p.timeout_ns, nullptr)
+                                              : mbar_wait(v_full(v_slot(j)), v_par(j), p.timeout_ns, nullptr);
         }
         if (!drained) attn_raise(p, abort_flag, kDevTimeoutDrain);
       }
@@ -433,6 +480,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (!mbar_wait(drain, 0u, p.timeout_ns, nullptr)) attn_raise(p, abort_flag, kDevTimeoutDrain);
       }
       __syncwarp();
+    } else if (kCross && clean_v) {
+      // ---- warps 10, 11: zero the V rows past the last key ---------------------
+      const int j = n_max - 1;
+      const bool got = mbar_wait(v_raw, 0u, p.timeout_ns, abort_flag);
+      if (__all_sync(0xffffffffu, got)) {
+        // A row is 128 bytes of each 64-column atom (the swizzle stays inside it).
+        const uint32_t tile = sV + (uint32_t)(v_slot(j) * Plan::kTileBytes);
+        const int cells = (kAttnBKV - (kv_len - j * kAttnBKV)) * 16;  // 16-byte cells, both atoms
+        for (int c = (warp - kAttnMmaWarp - 1) * 32 + (int)lane; c < cells; c += 64) {
+          const int row = kAttnBKV - 1 - (c >> 4);
+          const uint32_t dst = tile + (uint32_t)((row >> 6) * 16384 + ((c >> 3) & 1) * 8192 + (row & 63) * 128 + (c & 7) * 16);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
+        }
+        fence_proxy_async_smem();  // before the tensor cores read them
+      } else if (lane == 0) {
+        attn_raise(p, abort_flag, kDevTimeoutProducer);
+      }
+      named_bar_sync(1, 64);
+      if (warp == kAttnMmaWarp + 1 && lane == 0) mbar_arrive(v_full(v_slot(j)));
+      __syncwarp();
     }
   } else {
     setmaxnreg_inc<kAttnRegsSoftmax>();
@@ -473,9 +540,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const bool diag = p.causal && kv0 + kAttnBKV > qt * kAttnBQ;  // the tile crossing the diagonal
       // Only the diagonal tile and a tile past the sequence end need masks:
       // keys c >= lim are masked.
-      const bool masked = diag || kv0 + kAttnBKV > p.seq_len;
+      const bool masked = diag || kv0 + kAttnBKV > kv_len;
       if (masked) {
-        const int lim = min(p.seq_len - kv0, diag ? q_idx - kv0 + 1 : kAttnBKV);
+        const int lim = min(kv_len - kv0, diag ? q_idx - kv0 + 1 : kAttnBKV);
 #pragma unroll
         for (int c = 0; c < kAttnBKV; ++c) x[c] = c < lim ? x[c] : -INFINITY;
       }
@@ -537,6 +604,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (__all_sync(0xffffffffu, last)) {
         tc_fence_after();
         const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
+        if constexpr (kCross) {
+          if (p.lse != nullptr && q_idx < p.seq_len) {
+            p.lse[((size_t)bat * p.heads + head) * p.seq_len + q_idx] =
+                l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          }
+        }
         const uint32_t stage = sQ + (uint32_t)(tile * Plan::kTileBytes + qw * 8192);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
@@ -556,7 +629,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         if (lane == 0) {
           for (int half = 0; half < 2; ++half) {
-            tma_store_3d(&tmO, stage + (uint32_t)(half * 4096), col0 + 64 * half, qt * kAttnBQ + qw * 32, bat);
+            if constexpr (kCross) {
+              tma_store_4d(&tmO, stage + (uint32_t)(half * 4096), 64 * half, head, qt * kAttnBQ + qw * 32, bat);
+            } else {
+              tma_store_3d(&tmO, stage + (uint32_t)(half * 4096), col0 + 64 * half, qt * kAttnBQ + qw * 32, bat);
+            }
           }
           bulk_commit_group();
           bulk_wait_group_read<0>();
@@ -565,6 +642,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       } else if (lane == 0) {
         attn_raise(p, abort_flag, kDevTimeoutEpilogue);
       }
+    } else if (kCross && qt < p.num_q_tiles) {
+      // No keys: O = 0, lse = -inf.  (Q was not loaded: its buffer stages the zeros.)
+      const uint32_t stage = sQ + (uint32_t)(tile * Plan::kTileBytes + qw * 8192);
+      uint32_t zero[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) zero[i] = 0u;
+      stage_row64(zero, zero, false, stage, 0u, lane);
+      if (p.lse != nullptr && q_idx < p.seq_len) {
+        p.lse[((size_t)bat * p.heads + head) * p.seq_len + q_idx] = -INFINITY;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        for (int half = 0; half < 2; ++half) {
+          tma_store_4d(&tmO, stage, 64 * half, head, qt * kAttnBQ + qw * 32, bat);
+        }
+        bulk_commit_group();
+        bulk_wait_group_read<0>();
+      }
+      __syncwarp();
     }
   }
 

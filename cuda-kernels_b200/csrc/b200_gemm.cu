@@ -25,6 +25,7 @@
 #include "split_f32.cuh"
 #include "attn_sm100.cuh"
 #include "attn_sm100_pair.cuh"
+#include "device_info.h"
 #include "peer_bcast.h"
 
 namespace {
@@ -210,12 +211,12 @@ int init_device(int dev, DeviceState& st) {
     if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem) != cudaSuccess)
       return B200_ERR_CUDA;
   }
-  if (cudaFuncSetAttribute(b200::flash_attn_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(b200::flash_attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            b200::AttnSmemPlan::kAllocBytes) != cudaSuccess)
     return B200_ERR_CUDA;
   {
     cudaFuncAttributes fa{};
-    if (cudaFuncGetAttributes(&fa, b200::flash_attn_fwd_kernel) != cudaSuccess) return B200_ERR_CUDA;
+    if (cudaFuncGetAttributes(&fa, b200::flash_attn_fwd_kernel<false>) != cudaSuccess) return B200_ERR_CUDA;
     st.attn_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
   }
   if (cudaFuncSetAttribute(b200::flash_attn_fwd_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -696,6 +697,16 @@ int gemm_impl(const void* A, const void* B, void* C, int64_t M, int64_t N, int64
 
 }  // namespace
 
+namespace b200 {
+int device_info(DeviceInfo* out) {
+  DeviceState* st = nullptr;
+  const int rc = current_device_state(&st);
+  if (rc != B200_OK) return rc;
+  *out = DeviceInfo{st->sm_count, st->status_ptr, st->timeout_ns, g_encode};
+  return B200_OK;
+}
+}  // namespace b200
+
 extern "C" B200_API int b200_gemm_bf16(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K,
                                        int64_t lda, int64_t ldb, int64_t ldc, int b_layout, void* stream) {
   return gemm_impl(A, B, C, M, N, K, lda, ldb, ldc, b_layout, nullptr, 0, stream);
@@ -1025,7 +1036,7 @@ extern "C" B200_API int b200_flash_attn_bf16(const void* Q, const void* K, const
   cfg.stream = reinterpret_cast<cudaStream_t>(stream_);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, b200::flash_attn_fwd_kernel, tmQ, tmK, tmV, tmO, p) == cudaSuccess ? B200_OK
+  return cudaLaunchKernelEx(&cfg, b200::flash_attn_fwd_kernel<false>, tmQ, tmK, tmV, tmO, p) == cudaSuccess ? B200_OK
                                                                                                       : B200_ERR_CUDA;
 }
 
@@ -1070,7 +1081,8 @@ extern "C" B200_API int b200_gemm_status(void* stream_, uint32_t* device_bits) {
     return B200_ERR_CUDA;
   if (cudaStreamSynchronize(stream) != cudaSuccess) return B200_ERR_CUDA;
   if (device_bits != nullptr) *device_bits = bits;
-  return bits == 0 ? B200_OK : B200_ERR_DEVICE_TIMEOUT;
+  if (bits == 0) return B200_OK;
+  return (bits & ~(uint32_t)b200::kDevBadIndex) != 0 ? B200_ERR_DEVICE_TIMEOUT : B200_ERR_BAD_INDEX;
 }
 
 extern "C" B200_API int b200_gemm_set_timeout_ns(uint64_t timeout_ns) {
@@ -1138,6 +1150,7 @@ extern "C" B200_API const char* b200_gemm_strerror(int code) {
     case B200_ERR_DEVICE_TIMEOUT: return "device-side wait timed out";
     case B200_ERR_TOO_LARGE: return "dimension too large";
     case B200_ERR_SCRATCH_LIMIT: return "split-K scratch needed exceeds the 16 MiB static buffer of b200_gemm_bf16_noalloc";
+    case B200_ERR_BAD_INDEX: return "a block table entry or a length on the device is out of range";
     default: return "unknown error";
   }
 }

@@ -28,6 +28,7 @@ enum DeviceStatus : uint32_t {
   kDevWrongArch = 16u,        // a copy of the kernel built without sm_100a features ran
   kDevTimeoutSplitK = 32u,    // the last split-K part gave up waiting for a partial
   kDevTimeoutPeer = 64u,      // the producer gave up waiting for another GPU's data (exchange flags)
+  kDevBadIndex = 128u,        // a block table entry or a length on the device is out of range
 };
 
 // Kernel bodies use tcgen05/TMA, which exist only in the sm_100a feature set.
@@ -270,6 +271,24 @@ __device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
                    reinterpret_cast<uint64_t>(tmap)),
                "r"(x), "r"(y), "r"(z), "r"(src)
+               : "memory");
+}
+
+// 4-D tiled load / store (x innermost): strided attention operands, one head
+// (y) and one batch entry (w) per box.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int32_t y,
+                                            int32_t z, int32_t w, uint64_t l2_policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(l2_policy)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int32_t x, int32_t y, int32_t z,
+                                             int32_t w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(x), "r"(y), "r"(z), "r"(w), "r"(src)
                : "memory");
 }
 

@@ -1,0 +1,444 @@
+// Host side of attention to stored keys and values (include/b200_gemm.h):
+// the 8-bit cache, attention over it, and cross attention.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "attn_sm100.cuh"
+#include "attn_split_sm100.cuh"
+#include "b200_gemm.h"
+#include "device_info.h"
+#include "kv_cache_sm100.cuh"
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+constexpr int64_t kLim = 0x7fffffffLL;
+constexpr size_t kWsAlign = 256;
+
+// Cross attention: at most this many query rows per key/value head run split
+// along the keys (attn_split_kernel), more on the tcgen05 kernel.
+constexpr int64_t kSplitMaxRows = 64;
+
+using SplitKernel = void (*)(const CUtensorMap, const CUtensorMap, const b200::SplitAttnParams);
+struct SplitVariant {
+  SplitKernel kernel;
+  void (*join)(const b200::SplitAttnParams);
+  int smem;
+  size_t part_floats;
+};
+// [source: bf16, fp8][row tiles per CTA - 1]
+const SplitVariant kSplit[2][2] = {
+    {{b200::attn_split_kernel<false, 1>, b200::attn_join_kernel<1>, b200::SplitPlan<false, 1>::kAllocBytes,
+      b200::SplitPlan<false, 1>::kPartFloats},
+     {b200::attn_split_kernel<false, 2>, b200::attn_join_kernel<2>, b200::SplitPlan<false, 2>::kAllocBytes,
+      b200::SplitPlan<false, 2>::kPartFloats}},
+    {{b200::attn_split_kernel<true, 1>, b200::attn_join_kernel<1>, b200::SplitPlan<true, 1>::kAllocBytes,
+      b200::SplitPlan<true, 1>::kPartFloats},
+     {b200::attn_split_kernel<true, 2>, b200::attn_join_kernel<2>, b200::SplitPlan<true, 2>::kAllocBytes,
+      b200::SplitPlan<true, 2>::kPartFloats}}};
+
+struct StoredState {
+  std::once_flag once;
+  int init_rc = B200_OK;
+  bool cross_regs_ok = false;  // setmaxnreg shares match the binary (attn_sm100.cuh)
+  int split_ctas[2][2] = {};   // resident CTAs of each split variant on the whole GPU
+};
+StoredState g_stored[kMaxDevices];
+
+int init_stored(const b200::DeviceInfo& di, StoredState& st) {
+  if (cudaFuncSetAttribute(b200::flash_attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           b200::AttnSmemPlan::kAllocBytes) != cudaSuccess)
+    return B200_ERR_CUDA;
+  cudaFuncAttributes fa{};
+  if (cudaFuncGetAttributes(&fa, b200::flash_attn_fwd_kernel<true>) != cudaSuccess) return B200_ERR_CUDA;
+  st.cross_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
+  for (int f = 0; f < 2; ++f) {
+    for (int t = 0; t < 2; ++t) {
+      const SplitVariant& v = kSplit[f][t];
+      int per_sm = 0;
+      if (cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess ||
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.kernel, b200::kSplitThreads, v.smem) != cudaSuccess ||
+          per_sm < 1)
+        return B200_ERR_CUDA;
+      st.split_ctas[f][t] = per_sm * di.sm_count;
+    }
+  }
+  return B200_OK;
+}
+
+int current_state(b200::DeviceInfo* di, StoredState** out) {
+  const int rc = b200::device_info(di);
+  if (rc != B200_OK) return rc;
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return B200_ERR_CUDA;
+  StoredState& st = g_stored[dev];
+  std::call_once(st.once, [&] { st.init_rc = init_stored(*di, st); });
+  if (st.init_rc != B200_OK) return st.init_rc;
+  *out = &st;
+  return B200_OK;
+}
+
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// A strided operand [batch, tokens, heads, 128]: strides positive multiples
+// of 8 elements where the extent is above 1, below the tensor maps' 2^40
+// bytes; strides of extent 1 are replaced by a valid value.
+int check_view(const b200_attn_view* v, int64_t batch, int64_t tokens, int64_t heads, b200_attn_view* out) {
+  if (v == nullptr || v->data == nullptr) return B200_ERR_INVALID_ARG;
+  *out = *v;
+  const int64_t extent[3] = {batch, tokens, heads};
+  int64_t* stride[3] = {&out->batch_stride, &out->seq_stride, &out->head_stride};
+  for (int i = 0; i < 3; ++i) {
+    if (extent[i] <= 1) *stride[i] = b200::kKvD;
+    if (*stride[i] < b200::kKvD) return B200_ERR_INVALID_ARG;
+    if (*stride[i] % 8 != 0) return B200_ERR_ALIGNMENT;
+    if (*stride[i] >= (1LL << 39)) return B200_ERR_TOO_LARGE;
+  }
+  return aligned(v->data, 16) ? B200_OK : B200_ERR_ALIGNMENT;
+}
+
+// 4-D bf16 map {128, heads, tokens, batch}: boxes of 64 columns x box_rows tokens of one head, 128B swizzle.
+int encode_view(const b200::DeviceInfo& di, CUtensorMap* map, const b200_attn_view& v, int64_t batch, int64_t tokens,
+                int64_t heads, uint32_t box_rows, bool is_load) {
+  cuuint64_t dims[4] = {(cuuint64_t)b200::kKvD, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
+  cuuint64_t strides[3] = {(cuuint64_t)v.head_stride * 2, (cuuint64_t)v.seq_stride * 2, (cuuint64_t)v.batch_stride * 2};
+  cuuint32_t box[4] = {64, 1, box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = di.encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.data, dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               is_load ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
+}
+
+// The cache's codes as rows of 128 bytes; boxes of a page, at most a tile of keys.
+int encode_cache(const b200::DeviceInfo& di, CUtensorMap* map, void* codes, int64_t rows, int64_t page_size) {
+  cuuint64_t dims[2] = {(cuuint64_t)b200::kKvD, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)b200::kKvD};
+  cuuint32_t box[2] = {(cuuint32_t)b200::kKvD, (cuuint32_t)std::min<int64_t>(page_size, b200::kSplitKeys)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = di.encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
+}
+
+template <typename... Params, typename... Args>
+int launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return B200_OK;
+  cudaGetLastError();
+  return B200_ERR_CUDA;
+}
+
+int check_heads(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  if (batch < 0 || q_len < 0 || heads < 0 || kv_heads < 0) return B200_ERR_INVALID_ARG;
+  if (head_dim != b200::kKvD) return B200_ERR_INVALID_ARG;
+  if ((heads > 0 && kv_heads == 0) || (kv_heads > 0 && heads % kv_heads != 0)) return B200_ERR_INVALID_ARG;
+  if (batch > 65535 || heads > 65535 || heads * batch > kLim || q_len * heads > kLim) return B200_ERR_TOO_LARGE;
+  return B200_OK;
+}
+
+int check_cache(const b200_kv_cache* c) {
+  if (c == nullptr || c->num_pages < 0 || c->kv_heads < 0 || c->max_pages < 0) return B200_ERR_INVALID_ARG;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return B200_ERR_INVALID_ARG;
+  if (c->table_stride < c->max_pages) return B200_ERR_INVALID_ARG;
+  if (c->num_pages > kLim || c->kv_heads > 65535 || c->num_pages * c->kv_heads > kLim / c->page_size ||
+      c->max_pages > kLim / c->page_size)
+    return B200_ERR_TOO_LARGE;
+  return B200_OK;
+}
+
+int check_cache_pointers(const b200_kv_cache* c) {
+  if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr))
+    return B200_ERR_INVALID_ARG;
+  if (c->max_pages > 0 && c->block_table == nullptr) return B200_ERR_INVALID_ARG;
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) ||
+      !aligned(c->block_table, 4))
+    return B200_ERR_ALIGNMENT;
+  return B200_OK;
+}
+
+// Launch shape of the split kernel for a problem: fp8 or bf16 source, `rows`
+// query rows per key/value head.
+struct SplitPlanHost {
+  int variant;  // row tiles per CTA - 1
+  int64_t row_tiles;
+  int ctas;
+  bool cut;  // some segment can be longer than a tile: partial results need the workspace
+  size_t bytes;
+};
+int plan_split_attn(const StoredState& st, bool fp8, int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_len,
+                    SplitPlanHost* out) {
+  out->variant = rows <= 16 ? 0 : 1;
+  const int64_t tile = 16 * (out->variant + 1);
+  out->row_tiles = (rows + tile - 1) / tile;
+  const int64_t tiles = (kv_len + b200::kSplitKeys - 1) / b200::kSplitKeys;  // of the longest segment
+  const int64_t segs = kv_heads * out->row_tiles;
+  if (segs > kLim) return B200_ERR_TOO_LARGE;
+  const int64_t resident = st.split_ctas[fp8 ? 1 : 0][out->variant];
+  // One CTA per tile at most (in double: the product may pass 2^63).
+  const double most = (double)batch * (double)segs * (double)std::max<int64_t>(tiles, 1);
+  out->ctas = (int)std::min((double)resident, most);
+  out->cut = tiles > 1;
+  out->bytes = out->cut ? (size_t)out->ctas * (2 * kSplit[fp8 ? 1 : 0][out->variant].part_floats * sizeof(float) +
+                                               sizeof(int4))
+                        : 0;
+  out->bytes = (out->bytes + kWsAlign - 1) / kWsAlign * kWsAlign;
+  return B200_OK;
+}
+
+int run_split(const b200::DeviceInfo& di, const SplitPlanHost& plan, bool fp8, const CUtensorMap& tmK,
+              const CUtensorMap& tmV, b200::SplitAttnParams& p, void* workspace, size_t workspace_bytes,
+              cudaStream_t stream) {
+  const SplitVariant& v = kSplit[fp8 ? 1 : 0][plan.variant];
+  if (plan.bytes > 0) {
+    if (workspace == nullptr || workspace_bytes < plan.bytes) return B200_ERR_INVALID_ARG;
+    if (!aligned(workspace, kWsAlign)) return B200_ERR_ALIGNMENT;
+    p.part = static_cast<float*>(workspace);
+    p.desc = reinterpret_cast<int4*>(p.part + 2 * (size_t)plan.ctas * v.part_floats);
+  }
+  p.row_tiles = (int32_t)plan.row_tiles;
+  p.timeout_ns = di.timeout_ns;
+  p.status = di.status;
+  const int rc = launch(v.kernel, dim3((unsigned)plan.ctas), b200::kSplitThreads, v.smem, stream, tmK, tmV, p);
+  if (rc != B200_OK || !plan.cut) return rc;
+  const int rows = std::min<int>(p.rows, 16 * (plan.variant + 1));
+  return launch(v.join, dim3((unsigned)plan.ctas, (unsigned)((rows + 3) / 4)), 128, 0, stream, p);
+}
+
+bool scale_ok(float scale) { return scale > 0.0f && std::isfinite(scale); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+bool cross_splits(int64_t q_len, int64_t heads, int64_t kv_heads) {
+  return kv_heads > 0 && q_len * (heads / kv_heads) <= kSplitMaxRows;
+}
+
+}  // namespace
+
+extern "C" B200_API int b200_kv_cache_write(const b200_attn_view* k, const b200_attn_view* v, const b200_kv_cache* cache,
+                                            const int32_t* seq_lens, const int32_t* new_lens, int64_t batch,
+                                            int64_t new_max, int64_t head_dim, void* stream_) {
+  int rc = check_cache(cache);
+  if (rc != B200_OK) return rc;
+  if (batch < 0 || new_max < 0 || head_dim != b200::kKvD) return B200_ERR_INVALID_ARG;
+  if (batch > 65535 || new_max > kLim) return B200_ERR_TOO_LARGE;
+  if (batch == 0 || new_max == 0 || cache->kv_heads == 0) return B200_OK;
+  if (seq_lens == nullptr) return B200_ERR_INVALID_ARG;
+  if ((rc = check_cache_pointers(cache)) != B200_OK) return rc;
+  b200_attn_view kk, vv;
+  if ((rc = check_view(k, batch, new_max, cache->kv_heads, &kk)) != B200_OK) return rc;
+  if ((rc = check_view(v, batch, new_max, cache->kv_heads, &vv)) != B200_OK) return rc;
+  const int64_t page = cache->page_size;
+  // New tokens reach at most this many pages of a sequence (the first may hold older tokens).
+  const int64_t touched = std::min((new_max - 1 + page - 1) / page + 1, std::max<int64_t>(cache->max_pages, 1));
+  const int64_t blocks = batch * touched * cache->kv_heads * 2;
+  if (touched > kLim || blocks > kLim) return B200_ERR_TOO_LARGE;
+  b200::DeviceInfo di;
+  if ((rc = b200::device_info(&di)) != B200_OK) return rc;
+  b200::KvWriteParams p{};
+  const b200_attn_view* in[2] = {&kk, &vv};
+  for (int i = 0; i < 2; ++i) {
+    p.x[i] = static_cast<const __nv_bfloat16*>(in[i]->data);
+    p.x_batch[i] = in[i]->batch_stride;
+    p.x_seq[i] = in[i]->seq_stride;
+    p.x_head[i] = in[i]->head_stride;
+  }
+  p.cache[0] = static_cast<uint8_t*>(cache->k);
+  p.cache[1] = static_cast<uint8_t*>(cache->v);
+  p.scale[0] = cache->k_scale;
+  p.scale[1] = cache->v_scale;
+  p.table = cache->block_table;
+  p.table_stride = cache->table_stride;
+  p.seq_lens = seq_lens;
+  p.new_lens = new_lens;
+  p.new_max = (int32_t)new_max;
+  p.kv_heads = (int32_t)cache->kv_heads;
+  p.num_pages = (int32_t)cache->num_pages;
+  p.max_pages = (int32_t)cache->max_pages;
+  p.pages_touched = (int32_t)touched;
+  p.status = di.status;
+  void (*kernel)(const b200::KvWriteParams) = page == 16   ? b200::kv_cache_write_kernel<16>
+                                              : page == 32 ? b200::kv_cache_write_kernel<32>
+                                              : page == 64 ? b200::kv_cache_write_kernel<64>
+                                                           : b200::kv_cache_write_kernel<128>;
+  return launch(kernel, dim3((unsigned)blocks), b200::kKvWriteThreads, 0, reinterpret_cast<cudaStream_t>(stream_), p);
+}
+
+extern "C" B200_API int b200_cache_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t heads,
+                                                        const b200_kv_cache* cache, size_t* bytes) {
+  if (bytes == nullptr) return B200_ERR_INVALID_ARG;
+  *bytes = 0;
+  int rc = check_cache(cache);
+  if (rc != B200_OK) return rc;
+  if ((rc = check_heads(batch, q_len, heads, cache->kv_heads, b200::kKvD)) != B200_OK) return rc;
+  if (batch == 0 || q_len == 0 || heads == 0) return B200_OK;
+  b200::DeviceInfo di;
+  StoredState* st = nullptr;
+  if ((rc = current_state(&di, &st)) != B200_OK) return rc;
+  SplitPlanHost plan;
+  if ((rc = plan_split_attn(*st, true, batch, q_len * (heads / cache->kv_heads), cache->kv_heads,
+                            cache->max_pages * cache->page_size, &plan)) != B200_OK)
+    return rc;
+  *bytes = plan.bytes;
+  return B200_OK;
+}
+
+extern "C" B200_API int b200_cache_attn(const b200_attn_view* q, const b200_kv_cache* cache, const int32_t* seq_lens,
+                                        const int32_t* new_lens, const b200_attn_view* o, int64_t batch, int64_t q_len,
+                                        int64_t heads, int64_t head_dim, float scale, void* workspace,
+                                        size_t workspace_bytes, void* stream_) {
+  int rc = check_cache(cache);
+  if (rc != B200_OK) return rc;
+  if ((rc = check_heads(batch, q_len, heads, cache->kv_heads, head_dim)) != B200_OK) return rc;
+  if (!scale_ok(scale)) return B200_ERR_INVALID_ARG;
+  if (batch == 0 || q_len == 0 || heads == 0) return B200_OK;
+  if (seq_lens == nullptr) return B200_ERR_INVALID_ARG;
+  if ((rc = check_cache_pointers(cache)) != B200_OK) return rc;
+  b200_attn_view qq, oo;
+  if ((rc = check_view(q, batch, q_len, heads, &qq)) != B200_OK) return rc;
+  if ((rc = check_view(o, batch, q_len, heads, &oo)) != B200_OK) return rc;
+  b200::DeviceInfo di;
+  StoredState* st = nullptr;
+  if ((rc = current_state(&di, &st)) != B200_OK) return rc;
+  b200::SplitAttnParams p{};
+  p.batch = (int32_t)batch;
+  p.q_len = (int32_t)q_len;
+  p.heads = (int32_t)heads;
+  p.kv_heads = (int32_t)cache->kv_heads;
+  p.group = (int32_t)(heads / cache->kv_heads);
+  p.rows = p.q_len * p.group;
+  p.q = static_cast<const __nv_bfloat16*>(qq.data);
+  p.q_batch = qq.batch_stride, p.q_seq = qq.seq_stride, p.q_head = qq.head_stride;
+  p.o = static_cast<__nv_bfloat16*>(oo.data);
+  p.o_batch = oo.batch_stride, p.o_seq = oo.seq_stride, p.o_head = oo.head_stride;
+  p.scale_log2 = kLog2e * scale;
+  p.seq_lens = seq_lens;
+  p.new_lens = new_lens;
+  p.kv_len = (int32_t)(cache->num_pages == 0 ? 0 : cache->max_pages * cache->page_size);
+  p.page_size = (int32_t)cache->page_size;
+  p.num_pages = (int32_t)cache->num_pages;
+  p.table = cache->block_table;
+  p.table_stride = cache->table_stride;
+  p.k_scale = cache->k_scale;
+  p.v_scale = cache->v_scale;
+  SplitPlanHost plan;
+  if ((rc = plan_split_attn(*st, true, batch, p.rows, p.kv_heads, cache->max_pages * cache->page_size, &plan)) != B200_OK)
+    return rc;
+  CUtensorMap tmK{}, tmV{};
+  if (p.kv_len > 0) {
+    const int64_t rows = cache->num_pages * cache->kv_heads * cache->page_size;
+    if ((rc = encode_cache(di, &tmK, cache->k, rows, cache->page_size)) != B200_OK ||
+        (rc = encode_cache(di, &tmV, cache->v, rows, cache->page_size)) != B200_OK)
+      return rc;
+  }
+  return run_split(di, plan, true, tmK, tmV, p, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream_));
+}
+
+extern "C" B200_API int b200_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
+                                                        int64_t kv_heads, size_t* bytes) {
+  if (bytes == nullptr) return B200_ERR_INVALID_ARG;
+  *bytes = 0;
+  int rc = check_heads(batch, q_len, heads, kv_heads, b200::kKvD);
+  if (rc != B200_OK) return rc;
+  if (kv_len < 0) return B200_ERR_INVALID_ARG;
+  if (kv_len > kLim) return B200_ERR_TOO_LARGE;
+  if (batch == 0 || q_len == 0 || heads == 0 || !cross_splits(q_len, heads, kv_heads)) return B200_OK;
+  b200::DeviceInfo di;
+  StoredState* st = nullptr;
+  if ((rc = current_state(&di, &st)) != B200_OK) return rc;
+  SplitPlanHost plan;
+  if ((rc = plan_split_attn(*st, false, batch, q_len * (heads / kv_heads), kv_heads, kv_len, &plan)) != B200_OK) return rc;
+  *bytes = plan.bytes;
+  return B200_OK;
+}
+
+extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200_attn_view* k, const b200_attn_view* v,
+                                             const int32_t* kv_lens, const b200_attn_view* o, float* lse, int64_t batch,
+                                             int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads,
+                                             int64_t head_dim, float scale, void* workspace, size_t workspace_bytes,
+                                             void* stream_) {
+  int rc = check_heads(batch, q_len, heads, kv_heads, head_dim);
+  if (rc != B200_OK) return rc;
+  if (kv_len < 0 || !scale_ok(scale)) return B200_ERR_INVALID_ARG;
+  if (batch == 0 || q_len == 0 || heads == 0) return B200_OK;
+  if (kv_len > kLim - 128 || q_len > 65535LL * b200::kAttnBQ) return B200_ERR_TOO_LARGE;
+  b200_attn_view qq, kk{}, vv{}, oo;
+  if ((rc = check_view(q, batch, q_len, heads, &qq)) != B200_OK) return rc;
+  if ((rc = check_view(o, batch, q_len, heads, &oo)) != B200_OK) return rc;
+  if (kv_len > 0) {
+    if ((rc = check_view(k, batch, kv_len, kv_heads, &kk)) != B200_OK) return rc;
+    if ((rc = check_view(v, batch, kv_len, kv_heads, &vv)) != B200_OK) return rc;
+  }
+  if (!aligned(lse, 4) || !aligned(kv_lens, 4)) return B200_ERR_ALIGNMENT;
+  b200::DeviceInfo di;
+  StoredState* st = nullptr;
+  if ((rc = current_state(&di, &st)) != B200_OK) return rc;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  CUtensorMap tmK{}, tmV{};
+  if (cross_splits(q_len, heads, kv_heads)) {
+    b200::SplitAttnParams p{};
+    p.batch = (int32_t)batch;
+    p.q_len = (int32_t)q_len;
+    p.heads = (int32_t)heads;
+    p.kv_heads = (int32_t)kv_heads;
+    p.group = (int32_t)(heads / kv_heads);
+    p.rows = p.q_len * p.group;
+    p.q = static_cast<const __nv_bfloat16*>(qq.data);
+    p.q_batch = qq.batch_stride, p.q_seq = qq.seq_stride, p.q_head = qq.head_stride;
+    p.o = static_cast<__nv_bfloat16*>(oo.data);
+    p.o_batch = oo.batch_stride, p.o_seq = oo.seq_stride, p.o_head = oo.head_stride;
+    p.lse = lse;
+    p.scale_log2 = kLog2e * scale;
+    p.seq_lens = kv_lens;
+    p.kv_len = (int32_t)kv_len;
+    SplitPlanHost plan;
+    if ((rc = plan_split_attn(*st, false, batch, p.rows, kv_heads, kv_len, &plan)) != B200_OK) return rc;
+    if (kv_len > 0 && ((rc = encode_view(di, &tmK, kk, batch, kv_len, kv_heads, b200::kSplitKeys, true)) != B200_OK ||
+                       (rc = encode_view(di, &tmV, vv, batch, kv_len, kv_heads, b200::kSplitKeys, true)) != B200_OK))
+      return rc;
+    return run_split(di, plan, false, tmK, tmV, p, workspace, workspace_bytes, stream);
+  }
+  if (!st->cross_regs_ok) return B200_ERR_CUDA;  // built with another register count: never launch it
+  CUtensorMap tmQ, tmO;
+  if ((rc = encode_view(di, &tmQ, qq, batch, q_len, heads, b200::kAttnBQ, true)) != B200_OK ||
+      (rc = encode_view(di, &tmO, oo, batch, q_len, heads, 32, false)) != B200_OK)
+    return rc;
+  if (kv_len > 0) {
+    if ((rc = encode_view(di, &tmK, kk, batch, kv_len, kv_heads, b200::kAttnBKV, true)) != B200_OK ||
+        (rc = encode_view(di, &tmV, vv, batch, kv_len, kv_heads, 64, true)) != B200_OK)
+      return rc;
+  } else {
+    tmK = tmV = tmQ;  // not read
+  }
+  b200::AttnParams p{};
+  p.seq_len = (int32_t)q_len;
+  p.heads = (int32_t)heads;
+  p.batch = (int32_t)batch;
+  p.group = (int32_t)(heads / kv_heads);
+  p.num_q_tiles = (int32_t)((q_len + b200::kAttnBQ - 1) / b200::kAttnBQ);
+  p.scale_log2 = kLog2e * scale;
+  p.timeout_ns = di.timeout_ns;
+  p.status = di.status;
+  p.kv_len = (int32_t)kv_len;
+  p.kv_lens = kv_lens;
+  p.lse = lse;
+  return launch(b200::flash_attn_fwd_kernel<true>,
+                dim3((unsigned)(heads * batch), (unsigned)((p.num_q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles)),
+                b200::kAttnThreads, b200::AttnSmemPlan::kAllocBytes, stream, tmQ, tmK, tmV, tmO, p);
+}

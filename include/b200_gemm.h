@@ -49,6 +49,7 @@ extern "C" {
 #define B200_ERR_DEVICE_TIMEOUT 6    /* a kernel wait hit its time limit (see b200_gemm_status) */
 #define B200_ERR_TOO_LARGE 7         /* a dimension exceeds 2^31-1 */
 #define B200_ERR_SCRATCH_LIMIT 8     /* b200_gemm_bf16_noalloc: split-K scratch beyond its 16 MiB static buffer */
+#define B200_ERR_BAD_INDEX 9         /* a block table entry or a length on the device is out of range (see b200_gemm_status) */
 
 /* Layout of the B operand. */
 #define B200_B_NK 0 /* B stored [N,K] row-major (K contiguous): C = A * B^T.  The reference's layout. */
@@ -256,6 +257,98 @@ B200_API int b200_flash_attn_bf16(const void* Q, const void* K, const void* V, v
 #define B200_ATTN_KERNEL_SINGLE 1
 #define B200_ATTN_KERNEL_PAIR 2
 B200_API int b200_flash_attn_set_kernel(int which);
+
+/*
+ * A strided bf16 attention operand [batch, tokens, heads, 128]: strides in
+ * elements between batch entries, tokens and heads (positive multiples of 8
+ * where the extent is above 1; the last dimension is contiguous), data
+ * 16-byte aligned.
+ */
+typedef struct b200_attn_view {
+  void* data;
+  int64_t batch_stride, seq_stride, head_stride;
+} b200_attn_view;
+
+/*
+ * A paged key/value cache in 8 bits (e4m3): codes [num_pages, kv_heads,
+ * page_size, 128] and one fp32 scale per (page, key/value head), [num_pages,
+ * kv_heads]; a value is code x scale.  page_size is 16, 32, 64 or 128;
+ * num_pages * kv_heads * page_size <= 2^31 - 1.  Place j of sequence b is slot
+ * j % page_size of page block_table[b * table_stride + j / page_size].
+ * Codes 16-byte aligned, packed.
+ */
+typedef struct b200_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_pages, page_size, kv_heads;
+  const int32_t* block_table;  /* device, [batch, max_pages] */
+  int64_t table_stride, max_pages;
+} b200_kv_cache;
+
+/*
+ * Appends new keys and values to the cache.  Of sequence b, seq_lens[b]
+ * tokens long afterwards, the last new_lens[b] tokens are new (new_lens NULL:
+ * new_max of each); they are tokens 0 .. new_lens[b] - 1 of k and v's entry
+ * b ([batch, new_max, kv_heads, 128]).  A page's scale becomes the smallest
+ * power of two >= 2^-100 that brings the page within e4m3's 448; where it
+ * grows, the codes already in the page are rounded to the new scale; a page
+ * whose slot 0 is written starts afresh.  Slots behind the new tokens are left
+ * as they are.  NaN stays NaN and takes no part in a scale, an infinity
+ * counts as bf16's largest value and becomes the largest code.  No page may belong to two sequences that are written in
+ * one call.  A sequence whose lengths or pages are out of range is not written
+ * and is reported by b200_gemm_status (B200_ERR_BAD_INDEX).  Asynchronous; no
+ * allocation.  No reference counterpart (the reference's attention has no
+ * cache).
+ */
+B200_API int b200_kv_cache_write(const b200_attn_view* k, const b200_attn_view* v, const b200_kv_cache* cache,
+                                 const int32_t* seq_lens, const int32_t* new_lens, int64_t batch, int64_t new_max,
+                                 int64_t head_dim, void* stream);
+
+/*
+ * Attention of the newest tokens over the cache: O = softmax(scale Q K^T) V
+ * for q and o [batch, q_len, heads, 128].  Of sequence b (seq_lens[b] tokens,
+ * the new ones included and already written) the queries are its last
+ * new_lens[b] tokens (NULL: q_len): query t is at place seq_lens[b] -
+ * new_lens[b] + t and attends to the places up to its own.  Query rows past
+ * new_lens[b], and rows that see nothing, become 0.  heads a multiple of the
+ * cache's kv_heads (grouped as in b200_flash_attn_bf16).  scale > 0.  Scales
+ * of the cache must be within [2^-100, 2^100].  Lengths and pages out of range
+ * are clamped or skipped and reported by b200_gemm_status
+ * (B200_ERR_BAD_INDEX); the rows of such a sequence are unspecified.
+ * fp32 softmax and accumulation; results do not depend on timing.  The
+ * workspace (b200_cache_attn_workspace_bytes, 256-byte aligned, no
+ * initialisation) may not be shared by calls that can run at the same time.
+ * No reference counterpart.
+ */
+B200_API int b200_cache_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t heads, const b200_kv_cache* cache,
+                                             size_t* bytes);
+B200_API int b200_cache_attn(const b200_attn_view* q, const b200_kv_cache* cache, const int32_t* seq_lens,
+                             const int32_t* new_lens, const b200_attn_view* o, int64_t batch, int64_t q_len,
+                             int64_t heads, int64_t head_dim, float scale, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/*
+ * Cross attention: O = softmax(scale Q K^T) V over keys of another length
+ * (an encoder's states): q and o [batch, q_len, heads, 128], k and v [batch,
+ * kv_len, kv_heads, 128], grouped heads as in b200_flash_attn_bf16, no causal
+ * mask.  kv_lens (device, [batch], or NULL) are the keys of each batch entry,
+ * clamped to [0, kv_len]; what k and v hold behind them is not used.
+ * An entry without keys gets O = 0 and lse = -inf.  lse (fp32, [batch, heads,
+ * q_len], or NULL): natural log of the softmax denominator, which
+ * b200_cross_attn_bwd_bf16 needs.  scale > 0.  Few query rows per key/value
+ * head run split along the keys, others on the tcgen05 kernel of
+ * b200_flash_attn_bf16.  The workspace (b200_cross_attn_workspace_bytes, 0 for
+ * many) as in b200_cache_attn.  o may not overlap an input.  No reference
+ * counterpart (its operator has one length for queries and keys).
+ */
+B200_API int b200_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
+                                             int64_t kv_heads, size_t* bytes);
+B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200_attn_view* k, const b200_attn_view* v,
+                                  const int32_t* kv_lens, const b200_attn_view* o, float* lse, int64_t batch,
+                                  int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Element type of D for b200_gemm_bf16_ex. */
 #define B200_DTYPE_BF16 0
