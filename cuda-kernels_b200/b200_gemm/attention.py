@@ -263,3 +263,38 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: to
         return (o, lse) if return_lse else o
 
     return _on(q.device, stream, call)
+
+
+def cross_attn_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                        lse: torch.Tensor, *, kv_lens: torch.Tensor | None = None, scale: float | None = None,
+                        stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of cross_attn (b200_cross_attn_bwd_bf16), bf16, shaped like q, k and v.
+
+    out and lse are what cross_attn(..., return_lse=True) gave for the same q, k, v, kv_lens and scale; dout is the gradient
+    of out.  dk and dv are summed over the query heads of a group and 0 behind an entry's keys.  The sums run in a fixed
+    order: equal inputs give equal bits."""
+    views = [_view(name, t) for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout))]
+    batch, q_len, kv_len, heads, kv_heads = _cross_shapes(q, k, v)
+    for name, t in (("out", out), ("dout", dout)):
+        if t.shape != q.shape or t.device != q.device:
+            raise ValueError(f"{name} must be {tuple(q.shape)} on {q.device}, got {tuple(t.shape)} on {t.device}")
+    if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32:
+        raise TypeError("lse must be a float32 torch.Tensor")
+    if lse.shape != (batch, heads, q_len) or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous [{batch}, {heads}, {q_len}] on {q.device}, got {tuple(lse.shape)}")
+    lens = _lens("kv_lens", kv_lens, batch, q.device)
+    scale = _scale(scale)
+    lib = _lib.load()
+
+    def call(s, allocate):
+        grads = [allocate(t.shape, torch.bfloat16) for t in (q, k, v)]
+        n = ctypes.c_size_t(0)
+        _check(lib.b200_cross_attn_bwd_workspace_bytes(batch, q_len, heads, ctypes.byref(n)), "cross_attn_backward workspace")
+        ws, ptr = _workspace(allocate, n.value)
+        outs = [_view(name, t) for name, t in zip(("dq", "dk", "dv"), grads)]
+        rc = lib.b200_cross_attn_bwd_bf16(*views, lse.data_ptr(), lens, *outs, batch, q_len, kv_len, heads, kv_heads, HEAD_DIM,
+                                          scale, ptr, n.value, s)
+        _check(rc, f"cross_attn_backward batch={batch} q_len={q_len} kv_len={kv_len} heads={heads} kv_heads={kv_heads}")
+        return tuple(grads)
+
+    return _on(q.device, stream, call)

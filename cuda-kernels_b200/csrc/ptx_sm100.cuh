@@ -292,6 +292,14 @@ __device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int
                : "memory");
 }
 
+// `bytes` (a multiple of 16) of contiguous global memory -> this CTA's shared
+// memory (both 16-byte aligned), completion on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit_group() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }

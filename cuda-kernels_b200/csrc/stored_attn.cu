@@ -1,5 +1,5 @@
 // Host side of attention to stored keys and values (include/b200_gemm.h):
-// the 8-bit cache, attention over it, and cross attention.
+// the 8-bit cache, attention over it, cross attention and its gradients.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <mutex>
 
+#include "attn_bwd_sm100.cuh"
 #include "attn_sm100.cuh"
 #include "attn_split_sm100.cuh"
 #include "b200_gemm.h"
@@ -45,7 +46,7 @@ const SplitVariant kSplit[2][2] = {
 struct StoredState {
   std::once_flag once;
   int init_rc = B200_OK;
-  bool cross_regs_ok = false;  // setmaxnreg shares match the binary (attn_sm100.cuh)
+  bool cross_regs_ok = false, bwd_regs_ok = false;  // setmaxnreg shares match the binary (attn_sm100.cuh)
   int split_ctas[2][2] = {};   // resident CTAs of each split variant on the whole GPU
 };
 StoredState g_stored[kMaxDevices];
@@ -57,6 +58,11 @@ int init_stored(const b200::DeviceInfo& di, StoredState& st) {
   cudaFuncAttributes fa{};
   if (cudaFuncGetAttributes(&fa, b200::flash_attn_fwd_kernel<true>) != cudaSuccess) return B200_ERR_CUDA;
   st.cross_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
+  if (cudaFuncSetAttribute(b200::attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b200::kAttnBwdSmem) !=
+          cudaSuccess ||
+      cudaFuncGetAttributes(&fa, b200::attn_bwd_kernel) != cudaSuccess)
+    return B200_ERR_CUDA;
+  st.bwd_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
   for (int f = 0; f < 2; ++f) {
     for (int t = 0; t < 2; ++t) {
       const SplitVariant& v = kSplit[f][t];
@@ -441,4 +447,106 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
   return launch(b200::flash_attn_fwd_kernel<true>,
                 dim3((unsigned)(heads * batch), (unsigned)((p.num_q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles)),
                 b200::kAttnThreads, b200::AttnSmemPlan::kAllocBytes, stream, tmQ, tmK, tmV, tmO, p);
+}
+
+namespace {
+int64_t bwd_padded(int64_t q_len) { return (q_len + 127) / 128 * 128; }
+size_t bwd_bytes(int64_t batch, int64_t q_len, int64_t heads) {
+  return 2 * sizeof(float) * (size_t)(batch * heads) * (size_t)bwd_padded(q_len);
+}
+}  // namespace
+
+extern "C" B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t heads, size_t* bytes) {
+  if (bytes == nullptr) return B200_ERR_INVALID_ARG;
+  *bytes = 0;
+  const int rc = check_heads(batch, q_len, heads, heads, b200::kKvD);
+  if (rc != B200_OK) return rc;
+  *bytes = bwd_bytes(batch, q_len, heads);
+  return B200_OK;
+}
+
+extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const b200_attn_view* k, const b200_attn_view* v,
+                                                 const b200_attn_view* o, const b200_attn_view* dout, const float* lse,
+                                                 const int32_t* kv_lens, const b200_attn_view* dq,
+                                                 const b200_attn_view* dk, const b200_attn_view* dv, int64_t batch,
+                                                 int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, float scale, void* workspace, size_t workspace_bytes,
+                                                 void* stream_) {
+  int rc = check_heads(batch, q_len, heads, kv_heads, head_dim);
+  if (rc != B200_OK) return rc;
+  if (kv_len < 0 || !scale_ok(scale)) return B200_ERR_INVALID_ARG;
+  const bool queries = q_len > 0 && heads > 0, keys = kv_len > 0 && kv_heads > 0;
+  if (batch == 0 || (!queries && !keys)) return B200_OK;
+  const int64_t q_tiles = queries ? (q_len + 127) / 128 : 0, kv_tiles = keys ? (kv_len + 127) / 128 : 0;
+  const int64_t dkv_ctas = kv_tiles * kv_heads * batch, dq_ctas = q_tiles * heads * batch;
+  if (kv_len > kLim - 128 || q_len > kLim - 128 || dkv_ctas > kLim || dq_ctas > kLim - dkv_ctas ||
+      q_tiles * std::max<int64_t>(heads, 1) > kLim)
+    return B200_ERR_TOO_LARGE;
+  b200_attn_view qq{}, oo{}, dd{}, dqv{}, kk{}, vv{}, dkv{}, dvv{};
+  if (queries) {
+    if ((rc = check_view(q, batch, q_len, heads, &qq)) != B200_OK || (rc = check_view(o, batch, q_len, heads, &oo)) != B200_OK ||
+        (rc = check_view(dout, batch, q_len, heads, &dd)) != B200_OK ||
+        (rc = check_view(dq, batch, q_len, heads, &dqv)) != B200_OK)
+      return rc;
+    if (lse == nullptr) return B200_ERR_INVALID_ARG;
+    if (workspace == nullptr || workspace_bytes < bwd_bytes(batch, q_len, heads)) return B200_ERR_INVALID_ARG;
+    if (!aligned(workspace, kWsAlign)) return B200_ERR_ALIGNMENT;
+  }
+  if (keys && ((rc = check_view(k, batch, kv_len, kv_heads, &kk)) != B200_OK ||
+               (rc = check_view(v, batch, kv_len, kv_heads, &vv)) != B200_OK ||
+               (rc = check_view(dk, batch, kv_len, kv_heads, &dkv)) != B200_OK ||
+               (rc = check_view(dv, batch, kv_len, kv_heads, &dvv)) != B200_OK))
+    return rc;
+  if (!aligned(lse, 4) || !aligned(kv_lens, 4)) return B200_ERR_ALIGNMENT;
+  b200::DeviceInfo di;
+  StoredState* st = nullptr;
+  if ((rc = current_state(&di, &st)) != B200_OK) return rc;
+  if (!st->bwd_regs_ok) return B200_ERR_CUDA;  // built with another register count: never launch it
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  b200::AttnBwdMaps tm{};
+  if (queries && ((rc = encode_view(di, &tm.q, qq, batch, q_len, heads, 128, true)) != B200_OK ||
+                  (rc = encode_view(di, &tm.dout, dd, batch, q_len, heads, 128, true)) != B200_OK ||
+                  (rc = encode_view(di, &tm.dq, dqv, batch, q_len, heads, 32, false)) != B200_OK))
+    return rc;
+  if (keys && ((rc = encode_view(di, &tm.k, kk, batch, kv_len, kv_heads, 128, true)) != B200_OK ||
+               (rc = encode_view(di, &tm.v, vv, batch, kv_len, kv_heads, 128, true)) != B200_OK ||
+               (rc = encode_view(di, &tm.dk, dkv, batch, kv_len, kv_heads, 32, false)) != B200_OK ||
+               (rc = encode_view(di, &tm.dv, dvv, batch, kv_len, kv_heads, 32, false)) != B200_OK))
+    return rc;
+  b200::AttnBwdParams p{};
+  p.q_len = (int32_t)q_len;
+  p.kv_len = (int32_t)(keys ? kv_len : 0);
+  p.heads = (int32_t)heads;
+  p.kv_heads = (int32_t)kv_heads;
+  p.group = (int32_t)(kv_heads > 0 ? heads / kv_heads : 0);
+  p.batch = (int32_t)batch;
+  p.q_tiles = (int32_t)q_tiles;
+  p.kv_tiles = (int32_t)kv_tiles;
+  p.dkv_ctas = (int32_t)dkv_ctas;
+  p.kv_lens = kv_lens;
+  p.scale = scale;
+  p.scale_log2 = kLog2e * scale;
+  p.timeout_ns = di.timeout_ns;
+  p.status = di.status;
+  if (queries) {
+    p.lse2 = static_cast<float*>(workspace);
+    p.delta = p.lse2 + (size_t)(batch * heads) * (size_t)(q_tiles * 128);
+    b200::AttnBwdDeltaParams d{};
+    d.o = static_cast<const __nv_bfloat16*>(oo.data);
+    d.o_batch = oo.batch_stride, d.o_seq = oo.seq_stride, d.o_head = oo.head_stride;
+    d.dout = static_cast<const __nv_bfloat16*>(dd.data);
+    d.d_batch = dd.batch_stride, d.d_seq = dd.seq_stride, d.d_head = dd.head_stride;
+    d.lse = lse;
+    d.lse2 = p.lse2;
+    d.delta = p.delta;
+    d.q_len = p.q_len;
+    d.heads = p.heads;
+    d.padded = (int32_t)(q_tiles * 128);
+    const int64_t rows = batch * heads;
+    d.rows = (int32_t)rows;
+    const dim3 grid((unsigned)(q_tiles * 16), (unsigned)std::min<int64_t>(rows, 65535), (unsigned)((rows + 65534) / 65535));
+    if ((rc = launch(b200::attn_bwd_delta_kernel, grid, 256, 0, stream, d)) != B200_OK) return rc;
+  }
+  return launch(b200::attn_bwd_kernel, dim3((unsigned)(dkv_ctas + dq_ctas)), b200::kAttnThreads, b200::kAttnBwdSmem, stream,
+                tm, p);
 }

@@ -350,6 +350,23 @@ B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200_attn_view*
                                   int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                   float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Gradients of cross attention: dq, dk, dv (shaped like q, k, v) from dout
+ * (shaped like o) and the forward's o and lse.  dk and dv are sums over the
+ * query heads of a group, and 0 behind the keys of an entry.  bf16 operands
+ * and results, fp32 sums in a fixed order (no atomics).  The gradients may not
+ * overlap an input or each other.  Workspace:
+ * b200_cross_attn_bwd_workspace_bytes, as above.  No reference counterpart
+ * (the reference has no backward pass).
+ */
+B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t heads, size_t* bytes);
+B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const b200_attn_view* k, const b200_attn_view* v,
+                                      const b200_attn_view* o, const b200_attn_view* dout, const float* lse,
+                                      const int32_t* kv_lens, const b200_attn_view* dq, const b200_attn_view* dk,
+                                      const b200_attn_view* dv, int64_t batch, int64_t q_len, int64_t kv_len,
+                                      int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
 /* Element type of D for b200_gemm_bf16_ex. */
 #define B200_DTYPE_BF16 0
 #define B200_DTYPE_F32 1

@@ -109,6 +109,38 @@ def test_cross_attn_refusals():
     assert lib.b200_cross_attn_workspace_bytes(2, 1000, 500, 4, 2, ctypes.byref(n)) == _lib.B200_OK and n.value == 0
 
 
+def test_cross_attn_backward_refusals():
+    from b200_gemm import _lib
+    lib = _lib.load()
+
+    def call(q=None, dv=None, o=None, lse=FAKE, lens=None, batch=2, q_len=4, kv_len=5, heads=4, kv_heads=2, d=128, scale=0.1,
+             ws=FAKE, n=1 << 20):
+        x = _view()
+        return lib.b200_cross_attn_bwd_bf16(q or x, x, x, o or x, x, P(lse), P(lens), x, x, dv or x, batch, q_len, kv_len,
+                                            heads, kv_heads, d, scale, P(ws), n, None)
+
+    bad = _lib.B200_ERR_INVALID_ARG
+    assert call(d=64) == bad
+    assert call(heads=3) == bad
+    assert call(kv_len=-1) == bad
+    assert call(scale=math.nan) == bad
+    assert call(lse=None) == bad
+    assert call(ws=None) == bad
+    assert call(n=2 * 4 * 8 * 128 - 1) == bad
+    assert call(q=_view(data=None)) == bad
+    assert call(dv=_view(sh=64)) == bad
+    assert call(o=_view(data=FAKE + 8)) == _lib.B200_ERR_ALIGNMENT
+    assert call(ws=FAKE + 16) == _lib.B200_ERR_ALIGNMENT
+    assert call(lens=FAKE + 2) == _lib.B200_ERR_ALIGNMENT
+    assert call(kv_len=1 << 31) == _lib.B200_ERR_TOO_LARGE
+    assert call(batch=0) == _lib.B200_OK
+    assert call(q_len=0, kv_len=0) == _lib.B200_OK
+    n = ctypes.c_size_t(0)
+    assert lib.b200_cross_attn_bwd_workspace_bytes(2, 129, 4, ctypes.byref(n)) == _lib.B200_OK
+    assert n.value == 2 * 4 * 8 * 256  # two floats per query row, whole tiles
+    assert lib.b200_cross_attn_bwd_workspace_bytes(2, -1, 4, ctypes.byref(n)) == bad
+
+
 def test_status_text():
     from b200_gemm import _lib
     assert b"out of range" in _lib.load().b200_gemm_strerror(_lib.B200_ERR_BAD_INDEX)

@@ -487,6 +487,122 @@ def test_cross_refusals():
     _ok()
 
 
+# --- cross_attn_backward ---------------------------------------------------------------
+
+
+def _grad_check(q, k, v, do, lens=None, scale=None, dev=None):
+    dq, dk, dv, ddo = _on([q, k, v, do]) if dev is None else dev
+    dev_lens = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out, lse = b200_gemm.cross_attn(dq, dk, dv, kv_lens=dev_lens, scale=scale, return_lse=True)
+    grads = b200_gemm.cross_attn_backward(ddo, dq, dk, dv, out, lse, kv_lens=dev_lens, scale=scale)
+    _ok()
+    want = ref.cross_attn(q, k, v, lens, 128 ** -0.5 if scale is None else scale, do)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        _within(got, *want[name], name)
+    return grads
+
+
+@pytest.mark.parametrize("heads", [(2, 2), (8, 2), (3, 1)], ids=["mha", "gqa", "mqa"])
+@pytest.mark.parametrize("n", [1, 64, 127, 128, 129, 300, 640])
+@pytest.mark.parametrize("t", [1, 5, 64, 127, 128, 129, 300, 520])
+def test_backward_lengths(t, n, heads):
+    q, k, v = _cross_inputs(t * 1000 + n + 1, 2, t, n, *heads)
+    _grad_check(q, k, v, _randn(torch.Generator().manual_seed(t + n), *q.shape))
+
+
+@pytest.mark.parametrize("t", [1, 100, 300])
+def test_backward_ragged_sources(t):
+    """Lengths on the device, an empty source, NaN and infinities behind every source; dk and dv are 0 there."""
+    lens = [0, 1, 100, 128, 129, 383, 384]
+    q, k, v = _cross_inputs(t + 50, len(lens), t, 384, 4, 2)
+    do = _randn(torch.Generator().manual_seed(t), *q.shape)
+    dq, dk, dv = _grad_check(q, _spoil(k, lens), _spoil(v, lens), do, lens)
+    assert not bool(dq[0].any())
+    for i, m in enumerate(lens):
+        assert not bool(dk[i, m:].any()) and not bool(dv[i, m:].any())
+
+
+def test_backward_strides_and_scale():
+    g = torch.Generator().manual_seed(61)
+    q, kv = _randn(g, 2, 4, 200, 128).transpose(1, 2), _randn(g, 2, 150, 2, 2, 128)
+    do = _randn(g, 2, 200, 6, 128)[:, :, 1:5]
+    d = kv.to(DEV)
+    _grad_check(q, kv[:, :, 0], kv[:, :, 1], do, None, 0.07, (q.to(DEV), d[:, :, 0], d[:, :, 1], do.to(DEV)))
+
+
+def test_backward_empty_sides():
+    for t, n in ((0, 130), (130, 0)):
+        q, k, v = _cross_inputs(t, 2, t, n, 4, 2)
+        q, k, v = _on([q, k, v])
+        out, lse = b200_gemm.cross_attn(q, k, v, return_lse=True)
+        grads = b200_gemm.cross_attn_backward(torch.ones_like(out), q, k, v, out, lse)
+        _ok()
+        assert all(a.shape == b.shape and not bool(a.any()) for a, b in zip(grads, (q, k, v)))
+
+
+def test_backward_repeats_bit_for_bit():
+    q, k, v = _on(_cross_inputs(62, 2, 700, 900, 8, 2))
+    do = _randn(torch.Generator().manual_seed(63), *q.shape).to(DEV)
+    out, lse = b200_gemm.cross_attn(q, k, v, return_lse=True)
+    first = b200_gemm.cross_attn_backward(do, q, k, v, out, lse)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(first, b200_gemm.cross_attn_backward(do, q, k, v, out, lse)))
+    _ok()
+
+
+def test_backward_refusals():
+    q, k, v = _on(_cross_inputs(0, 2, 3, 5, 4, 2))
+    out, lse = b200_gemm.cross_attn(q, k, v, return_lse=True)
+    f = b200_gemm.cross_attn_backward
+    with pytest.raises(ValueError):
+        f(out[:, :2], q, k, v, out, lse)
+    with pytest.raises(ValueError):
+        f(out[:, :1].expand(2, 3, 4, 128), q, k, v, out, lse)  # a broadcast gradient is materialised by its owner
+    with pytest.raises(TypeError):
+        f(out, q, k, v, out, lse.double())
+    with pytest.raises(ValueError):
+        f(out, q, k, v, out, lse.transpose(1, 2))
+    with pytest.raises(ValueError):
+        f(out, q, k, v[:, :4], out, lse)
+    with pytest.raises(ValueError):
+        f(out, q, k, v, out, lse, scale=math.nan)
+    _ok()
+
+
+def test_training_step_captured_and_on_another_stream():
+    """Forward and backward in a captured graph, replayed with new inputs, and on a side stream."""
+    g = torch.Generator().manual_seed(64)
+    q, k, v = _cross_inputs(65, 2, 150, 200, 4, 2)
+    lens = [200, 70]
+    dev = _on([q, k, v, _randn(g, *q.shape)])
+    dev_lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def step(**kw):
+        out, lse = b200_gemm.cross_attn(*dev[:3], kv_lens=dev_lens, return_lse=True, **kw)
+        return out, *b200_gemm.cross_attn_backward(dev[3], *dev[:3], out, lse, kv_lens=dev_lens, **kw)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        new = [_randn(g, *t.shape) for t in dev]
+        for d, x in zip(dev, new):
+            d.copy_(x)
+        graph.replay()
+        graph.replay()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        on_side = step(stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+        _ok()
+        want = ref.cross_attn(*new[:3], lens, dout=new[3])
+        for name, a, b in zip(("out", "dq", "dk", "dv"), got, on_side):
+            _within(a, *want[name], name)
+            assert torch.equal(a, b)
+
+
 # --- streams, graphs, together -----------------------------------------------------------
 
 
