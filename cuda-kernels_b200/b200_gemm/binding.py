@@ -1,5 +1,5 @@
-"""Loaders for the prebuilt torch-extension bindings (bf16_matmul/matmul.cpp and
-flash_attn/flash_attn.cpp).
+"""Loaders for the prebuilt torch-extension bindings (bf16_matmul/matmul.cpp,
+flash_attn/flash_attn.cpp and flash_attn/stored_attn.cpp).
 
 The extensions are built in-tree by build.py and imported from their files, so
 no JIT cache is involved at run time.
@@ -38,4 +38,10 @@ def load_attn_binding():
     """Return the attention extension module: flash_attn_b200(Q, K, V, causal=True) and
     fa2_tma_lazy_rescale(Q, K, V) (causal, the reference operator's name)."""
     name, ext_dir, _ = EXTENSIONS[1]
+    return _load(name, ext_dir)
+
+
+def load_stored_attn_binding():
+    """Return the extension module behind attention.py: kv_cache_write, cache_attn, cross_attn, cross_attn_backward."""
+    name, ext_dir, _ = EXTENSIONS[2]
     return _load(name, ext_dir)

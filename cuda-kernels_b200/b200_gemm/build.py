@@ -7,6 +7,8 @@
                                        bf16_matmul/matmul.cpp binding
     flash_attn/b200_flash_attn_ext.so  torch extension mirroring the reference's
                                        flash_attn/flash_attn.cpp binding
+    flash_attn/b200_stored_attn_ext.so torch extension behind attention.py (8-bit cache, cross
+                                       attention)
 
 Every CUDA compile targets sm_100a explicitly
 (-gencode arch=compute_100a,code=sm_100a); nothing here depends on the GPU
@@ -32,6 +34,7 @@ EXT_NAME = "b200_matmul_ext"
 EXTENSIONS = [
     (EXT_NAME, EXT_DIR, "matmul.cpp"),
     ("b200_flash_attn_ext", os.path.join(ROOT, "flash_attn"), "flash_attn.cpp"),
+    ("b200_stored_attn_ext", os.path.join(ROOT, "flash_attn"), "stored_attn.cpp"),
 ]
 
 NVCC_FLAGS = [
@@ -108,7 +111,7 @@ def _build_one(name: str, ext_dir: str, source: str, force: bool, verbose: bool)
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> str:
-    """Build the torch-extension bindings (bf16_matmul/matmul.cpp, flash_attn/flash_attn.cpp) against the
+    """Build the torch-extension bindings (bf16_matmul/matmul.cpp, flash_attn/*.cpp) against the
     C-ABI library; returns the GEMM extension's path."""
     paths = [_build_one(n, d, s, force, verbose) for n, d, s in EXTENSIONS]
     return paths[0]

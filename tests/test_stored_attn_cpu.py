@@ -159,6 +159,30 @@ def test_python_checks_on_cpu():
         b200_gemm.kv_cache_write(x, x, x, x, x, x, x, x)
 
 
+def test_python_none_and_other_types_are_refused():
+    """None for a tensor raises (never crashes), in every place that can be reached without a GPU."""
+    import b200_gemm
+    x = torch.zeros((1, 2, 2, 128), dtype=torch.bfloat16)
+    for args in ((None, x, x), (x, None, x), (x, x, None), (3, x, x), ([1], x, x)):
+        with pytest.raises((TypeError, ValueError)):
+            b200_gemm.cross_attn(*args)
+    for i in range(8):
+        args = [x] * 8
+        args[i] = None
+        with pytest.raises((TypeError, ValueError)):
+            b200_gemm.kv_cache_write(*args)
+    for i in range(7):
+        args = [x] * 7
+        args[i] = None
+        with pytest.raises((TypeError, ValueError)):
+            b200_gemm.cache_attn(*args)
+    for i in range(6):
+        args = [x] * 6
+        args[i] = None
+        with pytest.raises((TypeError, ValueError)):
+            b200_gemm.cross_attn_backward(*args)
+
+
 def test_power_scale():
     assert ref.power_scale(0.0) == 2.0 ** -100
     assert ref.power_scale(448.0) == 1.0

@@ -340,6 +340,13 @@ def test_cache_refusals():
         attn(q, kc, vc, ks, vs, table, lens.long())
     with pytest.raises(TypeError):
         attn(q, kc, vc, ks, vs, table, None)
+    for i in range(7):
+        args = [q, kc, vc, ks, vs, table, lens]
+        args[i] = None
+        with pytest.raises(TypeError):
+            attn(*args)
+        with pytest.raises(TypeError):
+            write(k, k, *args[1:]) if i else write(None, k, *args[1:])
     with pytest.raises(ValueError):
         attn(q[:, :, :3], kc, vc, ks, vs, table, lens)
     with pytest.raises(ValueError):
@@ -558,6 +565,11 @@ def test_backward_refusals():
         f(out[:, :2], q, k, v, out, lse)
     with pytest.raises(ValueError):
         f(out[:, :1].expand(2, 3, 4, 128), q, k, v, out, lse)  # a broadcast gradient is materialised by its owner
+    for i in range(6):
+        args = [out, q, k, v, out, lse]
+        args[i] = None
+        with pytest.raises(TypeError):
+            f(*args)
     with pytest.raises(TypeError):
         f(out, q, k, v, out, lse.double())
     with pytest.raises(ValueError):
