@@ -32,7 +32,7 @@ struct SplitVariant {
   int smem;
   size_t part_floats;
 };
-// [source: bf16, fp8][row tiles per CTA - 1]
+// [source: bf16, fp8][row tiles per warp - 1]
 const SplitVariant kSplit[2][2] = {
     {{b200::attn_split_kernel<false, 1>, b200::attn_join_kernel<1>, b200::SplitPlan<false, 1>::kAllocBytes,
       b200::SplitPlan<false, 1>::kPartFloats},
@@ -122,11 +122,11 @@ int encode_view(const b200::DeviceInfo& di, CUtensorMap* map, const b200_attn_vi
   return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
 }
 
-// The cache's codes as rows of 128 bytes; boxes of a page, at most a tile of keys.
+// The cache's codes as rows of 128 bytes; boxes of a page, at most a unit of keys.
 int encode_cache(const b200::DeviceInfo& di, CUtensorMap* map, void* codes, int64_t rows, int64_t page_size) {
   cuuint64_t dims[2] = {(cuuint64_t)b200::kKvD, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)b200::kKvD};
-  cuuint32_t box[2] = {(cuuint32_t)b200::kKvD, (cuuint32_t)std::min<int64_t>(page_size, b200::kSplitKeys)};
+  cuuint32_t box[2] = {(cuuint32_t)b200::kKvD, (cuuint32_t)std::min<int64_t>(page_size, b200::SplitPlan<true, 1>::kKeys)};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = di.encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -182,10 +182,10 @@ int check_cache_pointers(const b200_kv_cache* c) {
 // Launch shape of the split kernel for a problem: fp8 or bf16 source, `rows`
 // query rows per key/value head.
 struct SplitPlanHost {
-  int variant;  // row tiles per CTA - 1
+  int variant;  // row tiles per warp - 1
   int64_t row_tiles;
   int ctas;
-  bool cut;  // some segment can be longer than a tile: partial results need the workspace
+  bool cut;  // some segment can be longer than a unit: partial results need the workspace
   size_t bytes;
 };
 int plan_split_attn(const StoredState& st, bool fp8, int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_len,
@@ -193,15 +193,16 @@ int plan_split_attn(const StoredState& st, bool fp8, int64_t batch, int64_t rows
   out->variant = rows <= 16 ? 0 : 1;
   const int64_t tile = 16 * (out->variant + 1);
   out->row_tiles = (rows + tile - 1) / tile;
-  const int64_t tiles = (kv_len + b200::kSplitKeys - 1) / b200::kSplitKeys;  // of the longest segment
+  const int64_t keys = fp8 ? b200::SplitPlan<true, 1>::kKeys : b200::SplitPlan<false, 1>::kKeys;
+  const int64_t units = (kv_len + keys - 1) / keys;  // of the longest segment
   const int64_t segs = kv_heads * out->row_tiles;
   if (segs > kLim) return B200_ERR_TOO_LARGE;
   const int64_t resident = st.split_ctas[fp8 ? 1 : 0][out->variant];
-  // One CTA per tile at most (in double: the product may pass 2^63).
-  const double most = (double)batch * (double)segs * (double)std::max<int64_t>(tiles, 1);
-  out->ctas = (int)std::min((double)resident, most);
-  out->cut = tiles > 1;
-  out->bytes = out->cut ? (size_t)out->ctas * (2 * kSplit[fp8 ? 1 : 0][out->variant].part_floats * sizeof(float) +
+  // One worker per unit at most (in double: the product may pass 2^63).
+  const double most = (double)batch * (double)segs * (double)std::max<int64_t>(units, 1);
+  out->ctas = (int)std::min((double)resident, std::ceil(most / b200::kSplitWarps));
+  out->cut = units > 1;
+  out->bytes = out->cut ? (size_t)(out->ctas * b200::kSplitWarps) * (2 * kSplit[fp8 ? 1 : 0][out->variant].part_floats * sizeof(float) +
                                                sizeof(int4))
                         : 0;
   out->bytes = (out->bytes + kWsAlign - 1) / kWsAlign * kWsAlign;
@@ -212,19 +213,23 @@ int run_split(const b200::DeviceInfo& di, const SplitPlanHost& plan, bool fp8, c
               const CUtensorMap& tmV, b200::SplitAttnParams& p, void* workspace, size_t workspace_bytes,
               cudaStream_t stream) {
   const SplitVariant& v = kSplit[fp8 ? 1 : 0][plan.variant];
+  const int workers = plan.ctas * b200::kSplitWarps;
   if (plan.bytes > 0) {
     if (workspace == nullptr || workspace_bytes < plan.bytes) return B200_ERR_INVALID_ARG;
     if (!aligned(workspace, kWsAlign)) return B200_ERR_ALIGNMENT;
     p.part = static_cast<float*>(workspace);
-    p.desc = reinterpret_cast<int4*>(p.part + 2 * (size_t)plan.ctas * v.part_floats);
+    p.desc = reinterpret_cast<int4*>(p.part + 2 * (size_t)workers * v.part_floats);
   }
   p.row_tiles = (int32_t)plan.row_tiles;
+  p.workers = workers;
   p.timeout_ns = di.timeout_ns;
   p.status = di.status;
   const int rc = launch(v.kernel, dim3((unsigned)plan.ctas), b200::kSplitThreads, v.smem, stream, tmK, tmV, p);
   if (rc != B200_OK || !plan.cut) return rc;
   const int rows = std::min<int>(p.rows, 16 * (plan.variant + 1));
-  return launch(v.join, dim3((unsigned)plan.ctas, (unsigned)((rows + 3) / 4)), 128, 0, stream, p);
+  const dim3 grid((unsigned)((workers + b200::kJoinWorkers - 1) / b200::kJoinWorkers),
+                  (unsigned)std::min(rows, b200::kJoinRowBlocks));
+  return launch(v.join, grid, 32 * b200::kJoinWarps, 0, stream, p);
 }
 
 bool scale_ok(float scale) { return scale > 0.0f && std::isfinite(scale); }
@@ -413,10 +418,11 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
     p.scale_log2 = kLog2e * scale;
     p.seq_lens = kv_lens;
     p.kv_len = (int32_t)kv_len;
+    constexpr uint32_t kBox = b200::SplitPlan<false, 1>::kKeys;
     SplitPlanHost plan;
     if ((rc = plan_split_attn(*st, false, batch, p.rows, kv_heads, kv_len, &plan)) != B200_OK) return rc;
-    if (kv_len > 0 && ((rc = encode_view(di, &tmK, kk, batch, kv_len, kv_heads, b200::kSplitKeys, true)) != B200_OK ||
-                       (rc = encode_view(di, &tmV, vv, batch, kv_len, kv_heads, b200::kSplitKeys, true)) != B200_OK))
+    if (kv_len > 0 && ((rc = encode_view(di, &tmK, kk, batch, kv_len, kv_heads, kBox, true)) != B200_OK ||
+                       (rc = encode_view(di, &tmV, vv, batch, kv_len, kv_heads, kBox, true)) != B200_OK))
       return rc;
     return run_split(di, plan, false, tmK, tmV, p, workspace, workspace_bytes, stream);
   }
