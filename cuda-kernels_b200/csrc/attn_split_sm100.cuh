@@ -11,13 +11,13 @@
 // them per warp): a 128-row tcgen05 tile would be at least 7/8 padding, and the
 // instruction rate is far from being the limit.
 //
-// Split: every warp is a worker of its own.  The units (32 or 16 keys) of all
+// Split: every warp is a worker of its own.  The units (32 keys) of all
 // (batch entry, key/value head, row tile) segments form one line, cut into
 // equal ranges, one per resident warp (the lengths are device data, so every
 // warp computes its cut).  A segment that lies within one range is finished
 // there; of the others each warp leaves a partial result (O, max, sum) in the
 // workspace, joined in a fixed order by attn_join_kernel: results do not
-// depend on timing.  A warp loads its units itself by TMA, kSplitStages ahead
+// depend on timing.  A warp loads its units itself by TMA, one or two ahead
 // and across segments, so there is no barrier between warps and the end of a
 // segment stalls one warp of the SM's twelve.  (Four warps sharing each
 // 64-key tile, a producer warp, and a merge through shared memory per segment:
@@ -30,7 +30,10 @@
 //
 // fp8: codes become fp16 exactly.  Q becomes fp16 after an exact power-of-two
 // scaling per row (largest value to 2^11: what fp16 cannot hold of a row is
-// below 2^-35 of its largest value), undone on the scores.  The value scale is
+// below 2^-35 of its largest value), undone on the scores.  (Scores by the e4m3
+// mma on the codes themselves, Q in two e4m3 parts: exact enough, but 145 us
+// against 105 on 64 sequences of up to 8192, as that mma converts its operands
+// inside on this chip.)  The value scale is
 // folded into P relative to the running maximum of (score + log2 scale), so
 // that O needs no second set of accumulators: P in fp16 is at most 2^14
 // whatever the scales, and what it cannot hold is below 2^-34 of the row's largest.
@@ -49,7 +52,6 @@ namespace b200 {
 
 constexpr int kSplitWarps = 4;  // workers per CTA
 constexpr int kSplitThreads = 32 * kSplitWarps;
-constexpr int kSplitStages = 2;
 // Beginning a segment (its queries, block table and scales) and handing its
 // rows out costs a warp about as much as two units: it counts as that in the
 // line, or workers with many short segments finish last (58 us against a
@@ -87,20 +89,25 @@ struct SplitAttnParams {
 
 template <bool kFp8, int kTiles>
 struct SplitPlan {
-  static constexpr int kKeys = kFp8 ? 32 : 16;  // keys per unit: 4 KiB of K and 4 KiB of V
-  static constexpr int kHalfBytes = 4096;
+  // 16 KiB of K and V per warp.  fp8: two units, each with a barrier.  bf16: one
+  // unit, K and V with a barrier each: K of the next unit loads while P V runs,
+  // V while its scores do (two units of 16 keys, with twice the boxes and waits
+  // per byte: 64 us against 58 on 32 sources of 200 to 2000 keys, 16 heads).
+  static constexpr int kKeys = 32;  // keys per unit
+  static constexpr int kHalfBytes = kKeys * kKvD * (kFp8 ? 1 : 2);
   static constexpr int kStageBytes = 2 * kHalfBytes;
+  static constexpr int kStages = kFp8 ? 2 : 1;
   static constexpr int kRows = 16 * kTiles;
   static constexpr int kCtasPerSm = kTiles == 1 ? 3 : 2;
   // Per warp: stages, then scales per stage (2 x (K scale, V scale, log2 of
   // it)), segment queue, barriers.
-  static constexpr int kOffScale = kSplitWarps * kSplitStages * kStageBytes;
-  static constexpr int kQueue = kSplitStages + 2;  // segments between the loads and the products
-  static constexpr int kOffQueue = kOffScale + kSplitWarps * kSplitStages * 32;
+  static constexpr int kOffScale = kSplitWarps * kStages * kStageBytes;
+  static constexpr int kQueue = kStages + 2;  // segments between the loads and the products
+  static constexpr int kOffQueue = kOffScale + kSplitWarps * kStages * 32;
   static constexpr int kOffPages = kOffQueue + kSplitWarps * kQueue * 32;  // 32 pages: scales and number
   static constexpr int kOffCursor = kOffPages + kSplitWarps * 32 * 16;
   static constexpr int kOffBar = kOffCursor + kSplitWarps * 64;
-  static constexpr int kOffAbort = kOffBar + kSplitWarps * kSplitStages * 8;
+  static constexpr int kOffAbort = kOffBar + kSplitWarps * 16;
   static constexpr int kBytes = kOffAbort + 16;
   static constexpr int kAllocBytes = kBytes + 1024;
   static constexpr size_t kPartFloats = (size_t)kRows * (kKvD + 2);
@@ -199,6 +206,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
 #else
   using Plan = SplitPlan<kFp8, kTiles>;
   constexpr int kKeys = Plan::kKeys;
+  constexpr int kStages = Plan::kStages;
   constexpr int kRows = Plan::kRows;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
@@ -206,15 +214,16 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
   uint8_t* base_ptr = smem_raw + (base - raw_u32);
   const int warp = (int)threadIdx.x >> 5;
   const int lane = (int)(threadIdx.x & 31u);
-  auto sK = [&](int s) { return base + (uint32_t)((warp * kSplitStages + s) * Plan::kStageBytes); };
+  auto sK = [&](int s) { return base + (uint32_t)((warp * kStages + s) * Plan::kStageBytes); };
   auto sV = [&](int s) { return sK(s) + (uint32_t)Plan::kHalfBytes; };
-  auto full = [&](int s) { return base + (uint32_t)Plan::kOffBar + 8u * (warp * kSplitStages + s); };
-  float4* scales = reinterpret_cast<float4*>(base_ptr + Plan::kOffScale) + warp * kSplitStages * 2;
+  // fp8: unit in stage s has landed; bf16: K (0) or V (1) has.
+  auto full = [&](int s) { return base + (uint32_t)Plan::kOffBar + 8u * (warp * 2 + s); };
+  float4* scales = reinterpret_cast<float4*>(base_ptr + Plan::kOffScale) + warp * kStages * 2;
   SplitSegment* queue = reinterpret_cast<SplitSegment*>(base_ptr + Plan::kOffQueue) + warp * Plan::kQueue;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffAbort);
 
   if (lane == 0) {
-    for (int s = 0; s < kSplitStages; ++s) mbar_init(full(s), 1);
+    for (int s = 0; s < 2; ++s) mbar_init(full(s), 1);
     if (warp == 0) *abort_flag = 0u;
     fence_mbar_init();
   }
@@ -372,7 +381,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
       if constexpr (kFp8) take(ld);
     }
     const SplitSegment& ld = queue[(segments - 1) % Plan::kQueue];
-    const int s = (int)(loaded % kSplitStages);
+    [[maybe_unused]] const int s = (int)(loaded % kStages);
     const int key0 = ld_t * kKeys;
     const int kv_head = ld.seg / p.row_tiles;
     if constexpr (kFp8) {
@@ -397,19 +406,32 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
         tma_load_2d(sV(s) + (uint32_t)(lane * box * kKvD), &tmV, full(s), 0, row, pol);
       }
     } else {
-      if (lane == 0) mbar_arrive_expect_tx(full(s), (uint32_t)Plan::kStageBytes);
+      if (lane == 0) mbar_arrive_expect_tx(full(0), (uint32_t)Plan::kHalfBytes);
       __syncwarp();
       if (lane < 2) {
-        tma_load_4d(sK(s) + (uint32_t)(lane * 2048), &tmK, full(s), 64 * lane, kv_head, key0, ld.b, pol);
-        tma_load_4d(sV(s) + (uint32_t)(lane * 2048), &tmV, full(s), 64 * lane, kv_head, key0, ld.b, pol);
+        tma_load_4d(sK(0) + (uint32_t)(lane * Plan::kHalfBytes / 2), &tmK, full(0), 64 * lane, kv_head, key0, ld.b, pol);
       }
     }
     ++ld_t;
     ++loaded;
     __syncwarp();  // the scales, before other lanes read them
   };
+  // bf16: V of the unit that load_next loaded K of, if it is not loaded yet.
+  [[maybe_unused]] uint32_t v_loaded = 0;
+  auto load_v = [&]() {
+    if (v_loaded == loaded) return;
+    const SplitSegment& ld = queue[(segments - 1) % Plan::kQueue];
+    if (lane == 0) mbar_arrive_expect_tx(full(1), (uint32_t)Plan::kHalfBytes);
+    __syncwarp();
+    if (lane < 2) {
+      tma_load_4d(sV(0) + (uint32_t)(lane * Plan::kHalfBytes / 2), &tmV, full(1), 64 * lane, ld.seg / p.row_tiles,
+                  (ld_t - 1) * kKeys, ld.b, pol);
+    }
+    ++v_loaded;
+  };
 #pragma unroll 1
-  for (int s = 0; s < kSplitStages; ++s) load_next();
+  for (int s = 0; s < kStages; ++s) load_next();
+  if constexpr (!kFp8) load_v();
 
   // ---- products and softmax -----------------------------------------------------------
   const int g = lane >> 2, t4 = lane & 3;
@@ -483,9 +505,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
     }
 
     for (int t = cur.t0; t < cur.t1; ++t, ++used) {
-      const int s = (int)(used % kSplitStages);
-      const bool got = mbar_wait(full(s), (used / kSplitStages) & 1u, p.timeout_ns, abort_flag);
-      ok = __all_sync(0xffffffffu, got);
+      const int s = (int)(used % kStages);
+      ok = __all_sync(0xffffffffu, mbar_wait(full(s), (used / kStages) & 1u, p.timeout_ns, abort_flag));
       if (!ok) break;
       const int key0 = t * kKeys;
       constexpr int kN = kKeys / 8;  // 8-key fragments of a unit
@@ -519,14 +540,20 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t cell = (uint32_t)(2 * (k & 3) + ((lane >> 3) & 1));
-          uint32_t r[4];
-          ldmatrix_x4(r, sK(s) + (uint32_t)((k >> 2) * 2048 + key * 128) + ((cell ^ (uint32_t)(key & 7)) << 4));
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) {
-            mma_bf16(x[m][0], qa[m][k], r[0], r[1]);
-            mma_bf16(x[m][1], qa[m][k], r[2], r[3]);
+          for (int f = 0; f < kKeys / 16; ++f) {
+            uint32_t r[4];
+            ldmatrix_x4(r, sK(0) + (uint32_t)((k >> 2) * (Plan::kHalfBytes / 2) + (16 * f + key) * 128) +
+                               ((cell ^ (uint32_t)(key & 7)) << 4));
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m) {
+              mma_bf16(x[m][2 * f], qa[m][k], r[0], r[1]);
+              mma_bf16(x[m][2 * f + 1], qa[m][k], r[2], r[3]);
+            }
           }
         }
+        __syncwarp();  // K is read: load the next unit's
+        load_next();
       }
       // Scales of the unit's 16-key halves.
       constexpr int kHalves = kKeys / 16;
@@ -639,11 +666,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
           }
         }
       } else {
+        ok = __all_sync(0xffffffffu, mbar_wait(full(1), used & 1u, p.timeout_ns, abort_flag));
+        if (!ok) break;
         if (cut) {
-          for (int c = lane; c < 16 * 16; c += 32) {
+          for (int c = lane; c < kKeys * 16; c += 32) {
             const int key = c >> 4;
             if (key0 + key >= len) {
-              const uint32_t dst = sV(s) + (uint32_t)(((c >> 3) & 1) * 2048 + key * 128 + (c & 7) * 16);
+              const uint32_t dst = sV(0) + (uint32_t)(((c >> 3) & 1) * (Plan::kHalfBytes / 2) + key * 128 + (c & 7) * 16);
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
             }
           }
@@ -652,20 +681,28 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
         // Blocks (keys 0-7, d 0-7), (keys 8-15, d 0-7), (keys 0-7, d 8-15), (keys 8-15, d 8-15).
         const int key = lane & 15;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t cell = (uint32_t)(2 * (j & 3) + (lane >> 4));
-          uint32_t r[4];
-          ldmatrix_x4_trans(r, sV(s) + (uint32_t)((j >> 2) * 2048 + key * 128) + ((cell ^ (uint32_t)(key & 7)) << 4));
+        for (int f = 0; f < kHalves; ++f) {
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) {
-            mma_bf16(o[m][2 * j], pa[m][0], r[0], r[1]);
-            mma_bf16(o[m][2 * j + 1], pa[m][0], r[2], r[3]);
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t cell = (uint32_t)(2 * (j & 3) + (lane >> 4));
+            uint32_t r[4];
+            ldmatrix_x4_trans(r, sV(0) + (uint32_t)((j >> 2) * (Plan::kHalfBytes / 2) + (16 * f + key) * 128) +
+                                     ((cell ^ (uint32_t)(key & 7)) << 4));
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m) {
+              mma_bf16(o[m][2 * j], pa[m][f], r[0], r[1]);
+              mma_bf16(o[m][2 * j + 1], pa[m][f], r[2], r[3]);
+            }
           }
         }
-        if (cut) fence_proxy_async_smem();  // the zeros, before TMA writes the stage again
+        if (cut) fence_proxy_async_smem();  // the zeros, before TMA writes there again
       }
-      __syncwarp();  // the stage is read: load into it
-      load_next();
+      __syncwarp();  // the stage (bf16: V) is read: load into it
+      if constexpr (kFp8) {
+        load_next();
+      } else {
+        load_v();
+      }
     }
     if (!ok) break;
 
@@ -731,8 +768,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitPlan<kFp8, kTiles>::kCtasP
     if (lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
     // Let the copies in flight land before the CTA can leave.
     bool drained = true;
-    for (uint32_t i = used; drained && i < loaded; ++i) {
-      drained = mbar_wait(full((int)(i % kSplitStages)), (i / kSplitStages) & 1u, p.timeout_ns, nullptr);
+    if constexpr (kFp8) {
+      for (uint32_t i = used; drained && i < loaded; ++i) {
+        drained = mbar_wait(full((int)(i % kStages)), (i / kStages) & 1u, p.timeout_ns, nullptr);
+      }
+    } else {
+      if (loaded > 0) drained = mbar_wait(full(0), (loaded - 1) & 1u, p.timeout_ns, nullptr);
+      if (drained && v_loaded > 0) drained = mbar_wait(full(1), (v_loaded - 1) & 1u, p.timeout_ns, nullptr);
     }
     if (!drained && lane == 0) attn_raise(p, abort_flag, kDevTimeoutDrain);
   }
