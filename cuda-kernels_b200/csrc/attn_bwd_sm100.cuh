@@ -5,7 +5,7 @@
 //
 // attn_bwd_delta_kernel writes delta and lse (in the exp2 domain) of every
 // query row, padded to whole tiles (+inf, 0: such rows get P = 0).
-// attn_bwd_kernel is one grid of two kinds of CTA, one per SM:
+// attn_bwd_kernel<kDQ> runs twice, persistent, one CTA per SM, over work items:
 //   dK/dV: one per 128-key tile, key/value head and batch entry, walking over
 //          the 128-row query tiles of every query head of the group;
 //   dQ:    one per 128-row query tile, head and batch entry, walking over the
@@ -13,10 +13,15 @@
 // Both recompute S and dP, 4 + 3 products a tile pair where a single pass
 // would need 5.  In exchange nothing is added across CTAs: the gradients of
 // shared heads are sums in a fixed order, with no atomics and no fp32
-// copy of dQ.  dK/dV CTAs come first in the grid (with grouped heads they are
-// the longer ones), dQ CTAs fill their last wave.
+// copy of dQ.  The dQ kernel starts on SMs that run out of dK/dV items.
+// Items are handed out by a counter (the delta kernel zeroes it), since their
+// lengths differ; the pipeline runs on from item to item: the next item's tiles load and its first
+// products run while the last one's gradients are stored.  (A CTA per item: 134
+// us against PPAIRS on 8 ragged pairs of 500 queries and up to 1333 keys, 16
+// heads, where an item has 4 to 11 tile pairs and start-up, epilogue and CTA
+// exchange took as long as those.)
 //
-// One body for both kinds.  X1, X2 are the CTA's own tiles, Y1, Y2 the
+// One body for both kinds.  X1, X2 are the item's own tiles, Y1, Y2 the
 // streamed ones; rows of the products are X's rows (TMEM lanes), columns Y's:
 //   dK/dV: X = K, V   Y = Q, dO   T1 = S^T, T2 = dP^T;  acc1 (dK) += dS^T Q, acc2 (dV) += P^T dO
 //   dQ:    X = Q, dO  Y = K, V    T1 = S,   T2 = dP;    acc1 (dQ) += dS K
@@ -24,13 +29,16 @@
 // every Y tile serves once as a K-major and once as an MN-major operand.
 //
 // 384 threads: warps 0..7 compute, two warpgroups of 64 columns each, one
-// thread per row; warp 8 TMA producer, warp 9 MMA issuer and TMEM owner, warps
-// 10, 11 zero the K rows past the last key in the last tile of a dQ CTA (they
-// may hold NaN, and 0 x NaN would reach dQ).
+// thread per row; warp 8 item fetch and TMA producer, warp 9 MMA issuer and
+// TMEM owner, warps 10, 11 (dQ) zero the K rows past the last key in an item's
+// last tile (they may hold NaN, and 0 x NaN would reach dQ).
 // TMEM, 512 columns: a warpgroup puts P and dS over its own half of T1, so no
 // warp waits for another.  dK/dV: T1 and T2 swap two regions from tile to
 // tile, T1 of the next tile being computed while dS of this one is.  dQ: T1
 // has two regions of its own, a tile ahead, T2 a third.
+// A steady tile pair takes 2.0 us in dK/dV and 1.5 in dQ, 0.49 us a product
+// either way: the rate at which this chip runs 128 x 128 x 128 products from one
+// CTA per SM, with or without the softmax (1300 TFLOP/s, as in the forward kernel).
 // Every wait is bounded, as in the forward kernel.
 #pragma once
 
@@ -44,21 +52,30 @@
 
 namespace b200 {
 
+// A gradient tensor [batch, tokens, heads, 128], strides in elements.
+struct AttnGrad {
+  __nv_bfloat16* data;
+  int64_t batch_stride, seq_stride, head_stride;
+};
+
 struct AttnBwdParams {
   int32_t q_len, kv_len, heads, kv_heads, group, batch;
   int32_t q_tiles, kv_tiles;
-  int32_t dkv_ctas;        // CTAs [0, dkv_ctas) compute dK and dV, the others dQ
+  int32_t items;           // of this kernel's kind
+  uint32_t early;          // dQ: launched behind the dK/dV kernel, of which it needs nothing
   const int32_t* kv_lens;  // [batch] or NULL
   float scale, scale_log2;
   // [batch * heads][q_tiles * 128], of attn_bwd_delta_kernel.
-  float* lse2;
-  float* delta;
+  const float* lse2;
+  const float* delta;
+  uint32_t* counter;       // items handed out beyond the first gridDim.x
+  AttnGrad dq, dk, dv;
   uint64_t timeout_ns;
   uint32_t* status;
 };
 
 struct AttnBwdMaps {
-  CUtensorMap q, k, v, dout, dq, dk, dv;
+  CUtensorMap q, k, v, dout;
 };
 
 struct AttnBwdDeltaParams {
@@ -71,35 +88,47 @@ struct AttnBwdDeltaParams {
   float* delta;
   int32_t q_len, heads, padded;  // padded = q_tiles * 128
   int32_t rows;                  // batch * heads
+  uint32_t* counters;            // two, zeroed for attn_bwd_kernel
 };
 
-// One warp per query row, 8 bytes of O and dO a lane: bound by reading both once.
+// Half a warp per query row, 16 bytes of O and dO a lane, four rows in flight
+// per half: bound by reading both once.
 __global__ void __launch_bounds__(256) attn_bwd_delta_kernel(const __grid_constant__ AttnBwdDeltaParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = (int)(threadIdx.x & 31u);
-  const int row = (int)blockIdx.x * 8 + ((int)threadIdx.x >> 5);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 2) p.counters[threadIdx.x] = 0u;
+  const int lane = (int)(threadIdx.x & 15u), sub = (int)threadIdx.x >> 4;
   const int bh = (int)blockIdx.y + 65535 * (int)blockIdx.z;
+  if (bh >= p.rows) return;
   const int head = bh % p.heads;
   const int64_t bat = bh / p.heads;
-  if (row >= p.padded || bh >= p.rows) return;
-  float sum = 0.0f, lse2 = INFINITY;
-  if (row < p.q_len) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p.o + bat * p.o_batch + row * p.o_seq + head * p.o_head + 4 * lane);
-    const uint2 b = *reinterpret_cast<const uint2*>(p.dout + bat * p.d_batch + row * p.d_seq + head * p.d_head + 4 * lane);
-    auto dot = [&](uint32_t x, uint32_t y) {
-      sum = fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), sum);
-      sum = fmaf(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u), sum);
-    };
-    dot(a.x, b.x);
-    dot(a.y, b.y);
+  // 64 rows per block: rows sub, sub + 16, sub + 32, sub + 48.
+  uint4 a[4], b[4];
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    lse2 = p.lse[(size_t)bh * p.q_len + row] * 1.4426950408889634f;
+  for (int i = 0; i < 4; ++i) {
+    const int row = (int)blockIdx.x * 64 + sub + 16 * i;
+    a[i] = b[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < p.q_len) {
+      a[i] = *reinterpret_cast<const uint4*>(p.o + bat * p.o_batch + row * p.o_seq + head * p.o_head + 8 * lane);
+      b[i] = *reinterpret_cast<const uint4*>(p.dout + bat * p.d_batch + row * p.d_seq + head * p.d_head + 8 * lane);
+    }
   }
-  if (lane == 0) {
-    p.lse2[(size_t)bh * p.padded + row] = lse2;
-    p.delta[(size_t)bh * p.padded + row] = sum;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (int)blockIdx.x * 64 + sub + 16 * i;
+    const uint32_t x[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, y[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      sum = fmaf(__uint_as_float(x[k] << 16), __uint_as_float(y[k] << 16), sum);
+      sum = fmaf(__uint_as_float(x[k] & 0xffff0000u), __uint_as_float(y[k] & 0xffff0000u), sum);
+    }
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (lane == 0 && row < p.padded) {
+      p.lse2[(size_t)bh * p.padded + row] = row < p.q_len ? p.lse[(size_t)bh * p.q_len + row] * 1.4426950408889634f : INFINITY;
+      p.delta[(size_t)bh * p.padded + row] = sum;
+    }
   }
 }
 
@@ -114,71 +143,116 @@ struct AttnBwdPlan {
   static constexpr int kOffY2 = kOffY1 + kY1Stages * kTileBytes;
   static constexpr int kOffVec = kOffY2 + kY2Stages * kTileBytes;  // dK/dV: lse2 and delta of a Y1 stage's rows
   static constexpr int kOffBar = kOffVec + (kDQ ? 0 : kY1Stages * 1024);
-  static constexpr int kNumBars = 2 + 2 * kY1Stages + 2 * kY2Stages + 2 + 1 + 1 + 1 + 2 + 2;
-  static constexpr int kOffTmemHolder = kOffBar + kNumBars * 8;
+  static constexpr int kNumBars = 2 + 3 * kY1Stages + 2 * kY2Stages + 2 + 1 + 1 + 1 + 2 + 1 + 1 + 4;
+  static constexpr int kOffItem = kOffBar + kNumBars * 8;  // two slots of (item or -1, keys of its entry)
+  static constexpr int kOffTmemHolder = kOffItem + 16;
   static constexpr int kOffAbort = kOffTmemHolder + 4;
   static constexpr int kBytes = kOffAbort + 4;
   static constexpr int kAllocBytes = kBytes + 1024;
   static_assert(kAllocBytes <= 232448, "attention backward shared memory plan exceeds 227 KiB");
 };
-constexpr int kAttnBwdSmem = AttnBwdPlan<true>::kAllocBytes > AttnBwdPlan<false>::kAllocBytes
-                                 ? AttnBwdPlan<true>::kAllocBytes
-                                 : AttnBwdPlan<false>::kAllocBytes;
+
+// 32 rows x 64 columns of a gradient, a row per lane in fp32 registers, scaled
+// by f: bf16, transposed within groups of eight lanes (three exchanges), so that eight
+// lanes store one row's 128 bytes.  (Each lane storing its own row, 16 bytes of 32
+// rows at a time, took 1.6 us a tile.)  Rows from `rows` on are not stored.
+__device__ __forceinline__ void store_grad(const AttnGrad& g, int bat, int row0, int rows, int head, int col, uint32_t lane,
+                                           const uint32_t (&lo)[32], const uint32_t (&hi)[32], float f) {
+  uint32_t w[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t* v = j < 4 ? &lo[8 * j] : &hi[8 * (j - 4)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[j][k] = pack_bf16x2(__uint_as_float(v[2 * k]) * f, __uint_as_float(v[2 * k + 1]) * f);
+  }
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) {
+    const bool upper = (lane & (uint32_t)d) != 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j & d) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[j][k] : w[j | d][k], d);
+        if (upper) {
+          w[j][k] = got;
+        } else {
+          w[j | d][k] = got;
+        }
+      }
+    }
+  }
+  const int first = row0 + (int)(lane & 24u);
+  __nv_bfloat16* dst = g.data + bat * g.batch_stride + first * g.seq_stride + head * g.head_stride + col + 8 * (lane & 7u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (first + j < rows) *reinterpret_cast<uint4*>(dst + j * g.seq_stride) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+  }
+}
 
 template <bool kDQ>
-__device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnBwdParams& p, int cta) {
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    attn_bwd_kernel(const __grid_constant__ AttnBwdMaps tm, const __grid_constant__ AttnBwdParams p) {
+#if B200_NO_SM100A_FEATURES
+  if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, (uint32_t)kDevWrongArch);
+#else
   using Plan = AttnBwdPlan<kDQ>;
   constexpr int S1 = Plan::kY1Stages, S2 = Plan::kY2Stages;
+  constexpr int kReaders = kDQ ? 11 : 9;  // of an item: MMA issuer, 8 computing warps, dQ: the two cleaning warps
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base = (raw_u32 + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - raw_u32);
   const uint32_t sX1 = base + Plan::kOffX1, sX2 = base + Plan::kOffX2;
-  auto sY1 = [&](int i) { return base + (uint32_t)(Plan::kOffY1 + (i % S1) * Plan::kTileBytes); };
-  auto sY2 = [&](int i) { return base + (uint32_t)(Plan::kOffY2 + (i % S2) * Plan::kTileBytes); };
+  // Tile pairs are counted over all of the CTA's items: g.
+  auto sY1 = [&](uint32_t g) { return base + (uint32_t)Plan::kOffY1 + (g % S1) * (uint32_t)Plan::kTileBytes; };
+  auto sY2 = [&](uint32_t g) { return base + (uint32_t)Plan::kOffY2 + (g % S2) * (uint32_t)Plan::kTileBytes; };
   const uint32_t bar0 = base + Plan::kOffBar;
-  const uint32_t x_full = bar0;
-  const uint32_t y1_raw = bar0 + 8u;  // dQ: the last K tile has landed, its rows past the last key not yet zero
-  auto y1_full = [&](int i) { return bar0 + 8u * (2 + i % S1); };
-  auto y1_empty = [&](int i) { return bar0 + 8u * (2 + S1 + i % S1); };
-  auto y2_full = [&](int i) { return bar0 + 8u * (2 + 2 * S1 + i % S2); };
-  auto y2_empty = [&](int i) { return bar0 + 8u * (2 + 2 * S1 + S2 + i % S2); };
-  auto y1_par = [](int i) { return (uint32_t)(i / S1) & 1u; };
-  auto y2_par = [](int i) { return (uint32_t)(i / S2) & 1u; };
-  constexpr int kB = 2 + 2 * S1 + 2 * S2;
-  auto t1_full = [&](int i) { return bar0 + 8u * (kB + (i & 1)); };
+  const uint32_t x_full = bar0, x_empty = bar0 + 8u;
+  auto y1_full = [&](uint32_t g) { return bar0 + 8u * (2 + g % S1); };
+  auto y1_empty = [&](uint32_t g) { return bar0 + 8u * (2 + S1 + g % S1); };
+  // dQ: an item's last K tile has landed, its rows past the last key not yet
+  // zero; y1_full then comes from the cleaning warps.  One per stage, and its
+  // phase counted by its uses: a stage is not used again before it was cleaned.
+  auto y1_raw = [&](uint32_t g) { return bar0 + 8u * (2 + 2 * S1 + g % S1); };
+  auto y2_full = [&](uint32_t g) { return bar0 + 8u * (2 + 3 * S1 + g % S2); };
+  auto y2_empty = [&](uint32_t g) { return bar0 + 8u * (2 + 3 * S1 + S2 + g % S2); };
+  auto y1_par = [](uint32_t g) { return (g / S1) & 1u; };
+  auto y2_par = [](uint32_t g) { return (g / S2) & 1u; };
+  constexpr int kB = 2 + 3 * S1 + 2 * S2;
+  auto t1_full = [&](uint32_t g) { return bar0 + 8u * (kB + (g & 1u)); };
   const uint32_t t2_full = bar0 + 8u * (kB + 2);
   const uint32_t t2_read = bar0 + 8u * (kB + 3);  // both warpgroups hold T2 in registers
   const uint32_t p_ready = bar0 + 8u * (kB + 4);
-  auto ds_ready = [&](int i) { return bar0 + 8u * (kB + 5 + (i & 1)); };
+  auto ds_ready = [&](uint32_t g) { return bar0 + 8u * (kB + 5 + (g & 1u)); };
   const uint32_t acc_full = bar0 + 8u * (kB + 7);
   const uint32_t drain = bar0 + 8u * (kB + 8);
+  auto item_full = [&](uint32_t k) { return bar0 + 8u * (kB + 9 + (k & 1u)); };
+  auto item_empty = [&](uint32_t k) { return bar0 + 8u * (kB + 11 + (k & 1u)); };
+  volatile int2* items = reinterpret_cast<volatile int2*>(base_ptr + Plan::kOffItem);
   volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffTmemHolder);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffAbort);
 
   const int warp = (int)threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
-  // This CTA's tile: dK/dV: key tile of a key/value head; dQ: query tile of a head.
-  const int own_tiles = kDQ ? p.q_tiles : p.kv_tiles;
-  const int own_heads = kDQ ? p.heads : p.kv_heads;
-  const int tile = cta % own_tiles;
-  const int head = (cta / own_tiles) % own_heads;
-  const int bat = (cta / own_tiles) / own_heads;
 
   if (warp == kAttnProducerWarp && lane == 0) {
     mbar_init(x_full, 1);
-    mbar_init(y1_raw, 1);
-    for (int s = 0; s < S1; ++s) {
+    mbar_init(x_empty, 1);
+    for (uint32_t s = 0; s < (uint32_t)S1; ++s) {
       mbar_init(y1_full(s), 1);
       mbar_init(y1_empty(s), 1);
+      mbar_init(y1_raw(s), 1);
     }
-    for (int s = 0; s < S2; ++s) {
+    for (uint32_t s = 0; s < (uint32_t)S2; ++s) {
       mbar_init(y2_full(s), 1);
       mbar_init(y2_empty(s), 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (uint32_t s = 0; s < 2; ++s) {
       mbar_init(t1_full(s), 1);
       mbar_init(ds_ready(s), 8);
+      mbar_init(item_full(s), 1);
+      mbar_init(item_empty(s), kReaders);
     }
     mbar_init(t2_full, 1);
     mbar_init(t2_read, 8);
@@ -187,6 +261,10 @@ __device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnB
     mbar_init(drain, 1);
     *abort_flag = 0u;
     fence_mbar_init();
+    tma_prefetch_desc(&tm.q);
+    tma_prefetch_desc(&tm.k);
+    tma_prefetch_desc(&tm.v);
+    tma_prefetch_desc(&tm.dout);
   }
   if (warp == kAttnMmaWarp) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_holder)), 512);
@@ -196,78 +274,138 @@ __device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnB
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  // The dK/dV kernel lets the next one start only after its own wait: a dQ CTA
+  // behind it then runs when all that came before both has completed, and
+  // needs no wait of its own (until the end, below).
+  if (!(kDQ && p.early != 0u)) pdl_wait();
   pdl_launch_dependents();
-  pdl_wait();
 
-  const int kv_len = attn_kv_len(p.kv_lens, bat, p.kv_len);
-  const int kv_tiles = (kv_len + 127) / 128;
-  // Streamed tiles: dK/dV: the query tiles of the group's heads, none for a
-  // key tile past the last key; dQ: the key tiles.
-  const int n = kDQ ? kv_tiles : (tile < kv_tiles ? p.group * p.q_tiles : 0);
-  // dQ: rows of the last K tile past the last key, which TMA filled from memory.
-  const bool clean = kDQ && kv_len < p.kv_len && kv_len % 128 != 0;
-  // TMEM regions of T1 and T2 of tile i (see the head of the file).
-  auto reg1 = [&](int i) { return tmem_base + (kDQ ? ((i & 1) ? 384u : 0u) : ((i & 1) ? 128u : 0u)); };
-  auto reg2 = [&](int i) { return tmem_base + (kDQ ? 128u : ((i & 1) ? 0u : 128u)); };
+  // An item: its tile, head and entry, and the number of tiles to stream.
+  struct Item {
+    int tile, head, bat, kv_len, n;
+    bool clean;  // dQ: rows of the last K tile past the last key, which TMA filled from memory
+  };
+  auto item_of = [&](int id, int kv_len) {
+    const int tiles = kDQ ? p.q_tiles : p.kv_tiles, heads = kDQ ? p.heads : p.kv_heads;
+    Item t;
+    t.tile = id % tiles;
+    t.head = (id / tiles) % heads;
+    t.bat = (id / tiles) / heads;
+    t.kv_len = kv_len;
+    const int kv_tiles = (kv_len + 127) / 128;
+    t.n = kDQ ? kv_tiles : (t.tile < kv_tiles ? p.group * p.q_tiles : 0);
+    t.clean = kDQ && kv_len < p.kv_len && kv_len % 128 != 0;
+    return t;
+  };
+  // The k-th item of this CTA, for one reader (a warp, or the MMA lane); false at the end.
+  auto next_item = [&](uint32_t k, bool whole_warp, Item* t, bool* ok) {
+    bool got = mbar_wait(item_full(k), (k >> 1) & 1u, p.timeout_ns, abort_flag);
+    if (whole_warp) got = __all_sync(0xffffffffu, got);
+    if (!got) {
+      *ok = false;
+      return false;
+    }
+    const int id = items[k & 1u].x, kv_len = items[k & 1u].y;
+    if (whole_warp) __syncwarp();
+    if (!whole_warp || lane == 0) mbar_arrive(item_empty(k));
+    if (id < 0) return false;
+    *t = item_of(id, kv_len);
+    return true;
+  };
+  // TMEM regions of T1 and T2 of tile pair g (see the head of the file).
+  auto reg1 = [&](uint32_t g) { return tmem_base + (kDQ ? ((g & 1u) ? 384u : 0u) : ((g & 1u) ? 128u : 0u)); };
+  auto reg2 = [&](uint32_t g) { return tmem_base + (kDQ ? 128u : ((g & 1u) ? 0u : 128u)); };
   const uint32_t acc1 = tmem_base + 256u;
   const uint32_t acc2 = tmem_base + 384u;  // dK/dV only
 
   if (warp >= kAttnProducerWarp) {
     setmaxnreg_dec<kAttnRegsOther>();
     if (warp == kAttnProducerWarp) {
-      // ---- TMA producer ------------------------------------------------------
-      if (lane == 0 && n > 0) {
+      // ---- item fetch and TMA producer ----------------------------------------
+      if (lane == 0) {
         const uint64_t pol_keep = l2_policy_evict_last();  // streamed tiles: read by many CTAs
         const uint64_t pol_once = l2_policy_evict_first();
-        auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int h, int row, uint64_t pol) {
-          for (int c = 0; c < 2; ++c) tma_load_4d(dst + (uint32_t)(c * 16384), map, bar, 64 * c, h, row, bat, pol);
-        };
-        mbar_arrive_expect_tx(x_full, 2 * Plan::kTileBytes);
-        load(sX1, kDQ ? &tm.q : &tm.k, x_full, head, tile * 128, pol_once);
-        load(sX2, kDQ ? &tm.dout : &tm.v, x_full, head, tile * 128, pol_once);
-        int y1_issued = 0, y2_issued = 0;
-        bool ok = true;
-        for (int i = 0; i < n; ++i) {
-          const int y_head = kDQ ? head / p.group : head * p.group + i / p.q_tiles;
-          const int y_row = (kDQ ? i : i % p.q_tiles) * 128;
-          if (!mbar_wait(y1_empty(i), y1_par(i) ^ 1u, p.timeout_ns, abort_flag)) {
+        uint32_t g = 0, filled = 0;  // tile pairs, items with tiles so far
+        uint32_t raw_par = 0;        // parity of each stage's next raw phase
+        bool ok = true, raw_last = false;
+        uint32_t y2_issued = 0;
+        int id = (int)blockIdx.x;
+        for (uint32_t k = 0;; ++k) {
+          if (!mbar_wait(item_empty(k), ((k >> 1) & 1u) ^ 1u, p.timeout_ns, abort_flag)) {
             ok = false;
             break;
           }
-          const uint32_t y1_bar = clean && i == n - 1 ? y1_raw : y1_full(i);
-          mbar_arrive_expect_tx(y1_bar, Plan::kTileBytes + (kDQ ? 0 : 1024));
-          load(sY1(i), kDQ ? &tm.k : &tm.q, y1_bar, y_head, y_row, pol_keep);
-          if constexpr (!kDQ) {
-            const size_t at = ((size_t)bat * p.heads + y_head) * (size_t)(p.q_tiles * 128) + y_row;
-            const uint32_t vec = base + (uint32_t)(Plan::kOffVec + (i % S1) * 1024);
-            bulk_load(vec, p.lse2 + at, 512, y1_bar);
-            bulk_load(vec + 512, p.delta + at, 512, y1_bar);
-          }
-          ++y1_issued;
-          if (!mbar_wait(y2_empty(i), y2_par(i) ^ 1u, p.timeout_ns, abort_flag)) {
+          const bool end = id >= p.items;
+          const int bat = end ? 0 : id / (kDQ ? p.q_tiles * p.heads : p.kv_tiles * p.kv_heads);
+          const int kv_len = end ? 0 : attn_kv_len(p.kv_lens, bat, p.kv_len);
+          items[k & 1u].x = end ? -1 : id;
+          items[k & 1u].y = kv_len;
+          mbar_arrive(item_full(k));
+          if (end) break;
+          const Item t = item_of(id, kv_len);
+          id = (int)(gridDim.x + atomicAdd(p.counter, 1u));  // the next one
+          if (t.n == 0) continue;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int h, int row, uint64_t pol) {
+            for (int c = 0; c < 2; ++c) tma_load_4d(dst + (uint32_t)(c * 16384), map, bar, 64 * c, h, row, t.bat, pol);
+          };
+          if (!mbar_wait(x_empty, (filled & 1u) ^ 1u, p.timeout_ns, abort_flag)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(y2_full(i), Plan::kTileBytes);
-          load(sY2(i), kDQ ? &tm.v : &tm.dout, y2_full(i), y_head, y_row, pol_keep);
-          ++y2_issued;
+          mbar_arrive_expect_tx(x_full, 2 * Plan::kTileBytes);
+          load(sX1, kDQ ? &tm.q : &tm.k, x_full, t.head, t.tile * 128, pol_once);
+          load(sX2, kDQ ? &tm.dout : &tm.v, x_full, t.head, t.tile * 128, pol_once);
+          ++filled;
+          for (int i = 0; i < t.n; ++i) {
+            const int y_head = kDQ ? t.head / p.group : t.head * p.group + i / p.q_tiles;
+            const int y_row = (kDQ ? i : i % p.q_tiles) * 128;
+            if (!mbar_wait(y1_empty(g), y1_par(g) ^ 1u, p.timeout_ns, abort_flag)) {
+              ok = false;
+              break;
+            }
+            raw_last = t.clean && i == t.n - 1;
+            const uint32_t y1_bar = raw_last ? y1_raw(g) : y1_full(g);
+            mbar_arrive_expect_tx(y1_bar, Plan::kTileBytes + (kDQ ? 0 : 1024));
+            load(sY1(g), kDQ ? &tm.k : &tm.q, y1_bar, y_head, y_row, pol_keep);
+            if constexpr (!kDQ) {
+              const size_t at = ((size_t)t.bat * p.heads + y_head) * (size_t)(p.q_tiles * 128) + y_row;
+              const uint32_t vec = base + (uint32_t)Plan::kOffVec + (g % S1) * 1024u;
+              bulk_load(vec, p.lse2 + at, 512, y1_bar);
+              bulk_load(vec + 512, p.delta + at, 512, y1_bar);
+            }
+            if (raw_last) raw_par ^= 1u << (g % S1);
+            ++g;
+            if (!mbar_wait(y2_empty(g - 1), y2_par(g - 1) ^ 1u, p.timeout_ns, abort_flag)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(y2_full(g - 1), Plan::kTileBytes);
+            load(sY2(g - 1), kDQ ? &tm.v : &tm.dout, y2_full(g - 1), y_head, y_row, pol_keep);
+            ++y2_issued;
+          }
+          if (!ok) break;
         }
         if (!ok) attn_raise(p, abort_flag, kDevTimeoutProducer);
-        // Let the copies in flight land before the CTA can leave.
-        bool drained = mbar_wait(x_full, 0u, p.timeout_ns, nullptr);
-        for (int i = y1_issued - 1; drained && i >= 0 && i >= y1_issued - S1; --i) {
-          drained = clean && i == n - 1 ? mbar_wait(y1_raw, 0u, p.timeout_ns, nullptr)
-                                        : mbar_wait(y1_full(i), y1_par(i), p.timeout_ns, nullptr);
+        // Let the copies in flight land before the CTA can leave.  (A raw tile
+        // other than the last was waited for by its cleaners, whose y1_full is
+        // waited for here.)
+        bool drained = filled == 0 || mbar_wait(x_full, (filled - 1) & 1u, p.timeout_ns, nullptr);
+        if (raw_last) {
+          drained = drained && mbar_wait(y1_raw(g - 1), ((raw_par >> ((g - 1) % S1)) & 1u) ^ 1u, p.timeout_ns, nullptr);
         }
-        for (int i = y2_issued - 1; drained && i >= 0 && i >= y2_issued - S2; --i) {
-          drained = mbar_wait(y2_full(i), y2_par(i), p.timeout_ns, nullptr);
+        for (uint32_t i = g; drained && i > 0 && i + S1 > g; --i) {
+          if (raw_last && i == g) continue;
+          drained = mbar_wait(y1_full(i - 1), y1_par(i - 1), p.timeout_ns, nullptr);
+        }
+        for (uint32_t i = y2_issued; drained && i > 0 && i + S2 > y2_issued; --i) {
+          drained = mbar_wait(y2_full(i - 1), y2_par(i - 1), p.timeout_ns, nullptr);
         }
         if (!drained) attn_raise(p, abort_flag, kDevTimeoutDrain);
       }
       __syncwarp();
     } else if (warp == kAttnMmaWarp) {
       // ---- MMA issuer ----------------------------------------------------------
-      if (lane == 0 && n > 0) {
+      if (lane == 0) {
         constexpr uint32_t idesc_t = idesc_bf16_f32(128, 128, false, false);  // X (K-major) x Y^T (K-major)
         constexpr uint32_t idesc_a = idesc_bf16_f32(128, 128, false, true);   // P or dS (TMEM) x Y (MN-major)
         auto kmajor = [](uint32_t t, int k) {
@@ -290,66 +428,96 @@ __device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnB
           tc_fence_after();
           return true;
         };
-        auto issue_t1 = [&](int i) {
-          if (!wait(y1_full(i), y1_par(i))) return false;
-          product(reg1(i), sX1, sY1(i));
-          umma_commit(t1_full(i));
+        auto issue_t1 = [&](uint32_t g) {
+          if (!wait(y1_full(g), y1_par(g))) return false;
+          product(reg1(g), sX1, sY1(g));
+          umma_commit(t1_full(g));
           return true;
         };
-        auto issue_t2 = [&](int i) {
-          if (!wait(y2_full(i), y2_par(i))) return false;
-          product(reg2(i), sX2, sY2(i));
+        // T2 is the last of a tile pair's products to read X.
+        auto issue_t2 = [&](uint32_t g, bool last) {
+          if (!wait(y2_full(g), y2_par(g))) return false;
+          product(reg2(g), sX2, sY2(g));
           umma_commit(t2_full);
-          if (kDQ) umma_commit(y2_empty(i));  // its only use
+          if (kDQ) umma_commit(y2_empty(g));  // its only use
+          if (last) umma_commit(x_empty);
           return true;
         };
-        auto run = [&]() {
-          if (!wait(x_full, 0u) || !issue_t1(0) || !issue_t2(0)) return false;
-          if (kDQ && n > 1 && !issue_t1(1)) return false;
+        auto run = [&](uint32_t g0, uint32_t filled, int n) {
+          if (!wait(x_full, filled & 1u) || !issue_t1(g0)) return false;
+          if (kDQ && n > 1 && !issue_t2(g0, false)) return false;
+          if (kDQ && n > 1 && !issue_t1(g0 + 1)) return false;
+          if (!(kDQ && n > 1) && !issue_t2(g0, n == 1)) return false;
           for (int i = 0; i < n; ++i) {
+            const uint32_t g = g0 + (uint32_t)i;
+            const bool next = i + 1 < n, next_last = i + 2 == n;
             if constexpr (kDQ) {
-              if (!wait(t2_read, (uint32_t)i & 1u)) return false;
-              if (i + 1 < n && !issue_t2(i + 1)) return false;
-              if (!wait(ds_ready(i), (uint32_t)(i >> 1) & 1u)) return false;
-              accumulate(acc1, reg1(i) + 32u, sY1(i), i == 0);
-              umma_commit(y1_empty(i));
-              if (i + 2 < n && !issue_t1(i + 2)) return false;
+              if (!wait(t2_read, g & 1u)) return false;
+              if (next && !issue_t2(g + 1, next_last)) return false;
+              if (!wait(ds_ready(g), (g >> 1) & 1u)) return false;
+              accumulate(acc1, reg1(g) + 32u, sY1(g), i == 0);
+              umma_commit(y1_empty(g));
+              if (i + 2 < n && !issue_t1(g + 2)) return false;
             } else {
-              if (!wait(p_ready, (uint32_t)i & 1u)) return false;
-              accumulate(acc2, reg1(i), sY2(i), i == 0);
-              umma_commit(y2_empty(i));
-              if (!wait(t2_read, (uint32_t)i & 1u)) return false;
-              if (i + 1 < n && !issue_t1(i + 1)) return false;
-              if (!wait(ds_ready(i), (uint32_t)(i >> 1) & 1u)) return false;
-              accumulate(acc1, reg1(i) + 32u, sY1(i), i == 0);
-              umma_commit(y1_empty(i));
-              if (i + 1 < n && !issue_t2(i + 1)) return false;
+              if (!wait(p_ready, g & 1u)) return false;
+              accumulate(acc2, reg1(g), sY2(g), i == 0);
+              umma_commit(y2_empty(g));
+              if (!wait(t2_read, g & 1u)) return false;
+              if (next && !issue_t1(g + 1)) return false;
+              if (!wait(ds_ready(g), (g >> 1) & 1u)) return false;
+              accumulate(acc1, reg1(g) + 32u, sY1(g), i == 0);
+              umma_commit(y1_empty(g));
+              if (next && !issue_t2(g + 1, next_last)) return false;
             }
           }
           umma_commit(acc_full);
           return true;
         };
-        if (!run()) attn_raise(p, abort_flag, kDevTimeoutMma);
+        bool ok = true;
+        uint32_t g = 0, filled = 0;
+        Item t;
+        for (uint32_t k = 0; ok && next_item(k, false, &t, &ok); ++k) {
+          if (t.n == 0) continue;
+          ok = run(g, filled, t.n);
+          g += (uint32_t)t.n;
+          ++filled;
+        }
+        if (!ok) attn_raise(p, abort_flag, kDevTimeoutMma);
         umma_commit(drain);
         if (!mbar_wait(drain, 0u, p.timeout_ns, nullptr)) attn_raise(p, abort_flag, kDevTimeoutDrain);
       }
       __syncwarp();
-    } else if (clean && n > 0) {
-      // ---- warps 10, 11: zero the K rows past the last key ---------------------
-      const bool got = mbar_wait(y1_raw, 0u, p.timeout_ns, abort_flag);
-      if (__all_sync(0xffffffffu, got)) {
-        const uint32_t t = sY1(n - 1);
-        const int cells = (128 * n - kv_len) * 16;  // 16-byte cells, both 64-column atoms
+    } else if (kDQ) {
+      // ---- warps 10, 11: zero the K rows past an item's last key ----------------
+      // Every decision is made by both warps together (a barrier that also
+      // carries it), so that neither waits for the other at a later one.
+      auto both = [&](bool mine) { return named_bar_and(1, 64, __all_sync(0xffffffffu, mine)); };
+      uint32_t g = 0, raw_par = 0;
+      bool ok = true;
+      for (uint32_t k = 0;; ++k) {
+        ok = both(mbar_wait(item_full(k), (k >> 1) & 1u, p.timeout_ns, abort_flag));
+        if (!ok) break;
+        const int id = items[k & 1u].x, kv_len = items[k & 1u].y;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty(k));
+        if (id < 0) break;
+        const Item t = item_of(id, kv_len);
+        g += (uint32_t)t.n;
+        if (!t.clean || t.n == 0) continue;
+        const uint32_t last = g - 1;
+        ok = both(mbar_wait(y1_raw(last), (raw_par >> (last % S1)) & 1u, p.timeout_ns, abort_flag));
+        if (!ok) break;
+        raw_par ^= 1u << (last % S1);
+        const int cells = (128 * t.n - t.kv_len) * 16;  // 16-byte cells, both 64-column atoms
         for (int c = (warp - kAttnMmaWarp - 1) * 32 + (int)lane; c < cells; c += 64) {
-          const uint32_t dst = t + (uint32_t)(((c >> 3) & 1) * 16384 + (127 - (c >> 4)) * 128 + (c & 7) * 16);
+          const uint32_t dst = sY1(last) + (uint32_t)(((c >> 3) & 1) * 16384 + (127 - (c >> 4)) * 128 + (c & 7) * 16);
           asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
         }
         fence_proxy_async_smem();  // before the tensor cores read them
-      } else if (lane == 0) {
-        attn_raise(p, abort_flag, kDevTimeoutProducer);
+        both(true);
+        if (warp == kAttnMmaWarp + 1 && lane == 0) mbar_arrive(y1_full(last));
       }
-      named_bar_sync(1, 64);
-      if (warp == kAttnMmaWarp + 1 && lane == 0) mbar_arrive(y1_full(n - 1));
+      if (!ok && lane == 0) attn_raise(p, abort_flag, kDevTimeoutProducer);
       __syncwarp();
     }
   } else {
@@ -359,15 +527,6 @@ __device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnB
     const int row = qw * 32 + (int)lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t half = lane_off + (uint32_t)(wg * 64);
-    float row_lse = 0.0f, row_delta = 0.0f;  // dQ: of this thread's query row
-    if constexpr (kDQ) {
-      const size_t at = ((size_t)bat * p.heads + head) * (size_t)(p.q_tiles * 128) + tile * 128 + row;
-      row_lse = p.lse2[at];
-      row_delta = p.delta[at];
-    }
-    // dK/dV: rows past the last key hold whatever memory holds: P = dS = 0.
-    const bool partial = !kDQ && tile * 128 + 128 > kv_len;
-    const bool row_ok = kDQ || tile * 128 + row < kv_len;
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t par) {
       const bool got = mbar_wait(bar, par, p.timeout_ns, abort_flag);
@@ -380,126 +539,133 @@ __device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnB
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    for (int i = 0; i < n; ++i) {
-      if (!wait(t1_full(i), (uint32_t)(i >> 1) & 1u)) break;
-      float e[64];
-      {
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(reg1(i) + half, r[0]);
-        tmem_ld_32x32b_x32(reg1(i) + half + 32u, r[1]);
-        tmem_ld_wait_regs(r[0]);
-        tmem_ld_wait_regs(r[1]);
-#pragma unroll
-        for (int c = 0; c < 64; ++c) e[c] = __uint_as_float(r[c >> 5][c & 31]);
+    uint32_t g0 = 0, filled = 0;
+    Item t;
+    for (uint32_t k = 0; ok && next_item(k, true, &t, &ok); ++k) {
+      const int kv_len = t.kv_len, n = t.n;
+      float row_lse = 0.0f, row_delta = 0.0f;  // dQ: of this thread's query row
+      if constexpr (kDQ) {
+        const size_t at = ((size_t)t.bat * p.heads + t.head) * (size_t)(p.q_tiles * 128) + t.tile * 128 + row;
+        row_lse = p.lse2[at];
+        row_delta = p.delta[at];
       }
-      const float* vec = reinterpret_cast<const float*>(base_ptr + Plan::kOffVec + (i % S1) * 1024) + wg * 64;
-      if constexpr (!kDQ) {
-        // The vectors came with Y1: the wait makes them visible to this thread.
-        if (!wait(y1_full(i), y1_par(i))) break;
-      }
+      // dK/dV: rows past the last key hold whatever memory holds: P = dS = 0.
+      const bool partial = !kDQ && t.tile * 128 + 128 > kv_len;
+      const bool row_ok = kDQ || t.tile * 128 + row < kv_len;
+      for (int i = 0; i < n; ++i) {
+        const uint32_t g = g0 + (uint32_t)i;
+        if (!wait(t1_full(g), (g >> 1) & 1u)) break;
+        float e[64];
+        {
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(reg1(g) + half, r[0]);
+          tmem_ld_32x32b_x32(reg1(g) + half + 32u, r[1]);
+          tmem_ld_wait_regs(r[0]);
+          tmem_ld_wait_regs(r[1]);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        float4 l4 = make_float4(row_lse, row_lse, row_lse, row_lse);
-        if constexpr (!kDQ) l4 = *reinterpret_cast<const float4*>(vec + c);
-        const float2 sc = make_float2(p.scale_log2, p.scale_log2);
-        const float2 a = __ffma2_rn(make_float2(e[c], e[c + 1]), sc, make_float2(-l4.x, -l4.y));
-        const float2 b = __ffma2_rn(make_float2(e[c + 2], e[c + 3]), sc, make_float2(-l4.z, -l4.w));
-        e[c] = fast_exp2(a.x);
-        e[c + 1] = fast_exp2(a.y);
-        e[c + 2] = fast_exp2(b.x);
-        e[c + 3] = fast_exp2(b.y);
-      }
-      if (kDQ && i == n - 1 && n * 128 > kv_len) {
-        const int lim = kv_len - i * 128 - wg * 64;
-#pragma unroll
-        for (int c = 0; c < 64; ++c) e[c] = c < lim ? e[c] : 0.0f;
-      }
-      if constexpr (!kDQ) {
-        if (partial) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) e[c] = row_ok ? e[c] : 0.0f;
+          for (int c = 0; c < 64; ++c) e[c] = __uint_as_float(r[c >> 5][c & 31]);
         }
-        uint32_t pw[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) pw[c] = pack_bf16x2(e[2 * c], e[2 * c + 1]);
-        tmem_st_32x32b_x32(reg1(i) + half, pw);
-        tmem_st_wait();
-        publish(p_ready);
-      }
-      if (!wait(t2_full, (uint32_t)i & 1u)) break;
-      uint32_t dw[32];
-      {
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(reg2(i) + half, r[0]);
-        tmem_ld_32x32b_x32(reg2(i) + half + 32u, r[1]);
-        tmem_ld_wait_regs(r[0]);
-        tmem_ld_wait_regs(r[1]);
-        publish(t2_read);
+        const float* vec = reinterpret_cast<const float*>(base_ptr + Plan::kOffVec + (g % S1) * 1024u) + wg * 64;
+        if constexpr (!kDQ) {
+          // The vectors came with Y1: the wait makes them visible to this thread.
+          if (!wait(y1_full(g), y1_par(g))) break;
+        }
 #pragma unroll
         for (int c = 0; c < 64; c += 4) {
-          float4 d4 = make_float4(row_delta, row_delta, row_delta, row_delta);
-          if constexpr (!kDQ) d4 = *reinterpret_cast<const float4*>(vec + 128 + c);
-          const uint32_t* t = &r[c >> 5][c & 31];
-          const float2 a = __fmul2_rn(make_float2(e[c], e[c + 1]),
-                                      __fadd2_rn(make_float2(__uint_as_float(t[0]), __uint_as_float(t[1])), make_float2(-d4.x, -d4.y)));
-          const float2 b = __fmul2_rn(make_float2(e[c + 2], e[c + 3]),
-                                      __fadd2_rn(make_float2(__uint_as_float(t[2]), __uint_as_float(t[3])), make_float2(-d4.z, -d4.w)));
-          dw[c >> 1] = pack_bf16x2(a.x, a.y);
-          dw[(c >> 1) + 1] = pack_bf16x2(b.x, b.y);
+          float4 l4 = make_float4(row_lse, row_lse, row_lse, row_lse);
+          if constexpr (!kDQ) l4 = *reinterpret_cast<const float4*>(vec + c);
+          const float2 sc = make_float2(p.scale_log2, p.scale_log2);
+          const float2 a = __ffma2_rn(make_float2(e[c], e[c + 1]), sc, make_float2(-l4.x, -l4.y));
+          const float2 b = __ffma2_rn(make_float2(e[c + 2], e[c + 3]), sc, make_float2(-l4.z, -l4.w));
+          e[c] = fast_exp2(a.x);
+          e[c + 1] = fast_exp2(a.y);
+          e[c + 2] = fast_exp2(b.x);
+          e[c + 3] = fast_exp2(b.y);
         }
-      }
-      // 0 x (NaN - delta): masked places again, on the packed pairs.
-      if (kDQ && i == n - 1 && n * 128 > kv_len) {
-        const int lim = kv_len - i * 128 - wg * 64;
+        if (kDQ && i == n - 1 && n * 128 > kv_len) {
+          const int lim = kv_len - i * 128 - wg * 64;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          dw[c] &= (2 * c < lim ? 0xffffu : 0u) | (2 * c + 1 < lim ? 0xffff0000u : 0u);
+          for (int c = 0; c < 64; ++c) e[c] = c < lim ? e[c] : 0.0f;
         }
-      }
-      if (partial) {
+        if constexpr (!kDQ) {
+          if (partial) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) dw[c] = row_ok ? dw[c] : 0u;
+            for (int c = 0; c < 64; ++c) e[c] = row_ok ? e[c] : 0.0f;
+          }
+          uint32_t pw[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pw[c] = pack_bf16x2(e[2 * c], e[2 * c + 1]);
+          tmem_st_32x32b_x32(reg1(g) + half, pw);
+          tmem_st_wait();
+          publish(p_ready);
+        }
+        if (!wait(t2_full, g & 1u)) break;
+        uint32_t dw[32];
+        {
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(reg2(g) + half, r[0]);
+          tmem_ld_32x32b_x32(reg2(g) + half + 32u, r[1]);
+          tmem_ld_wait_regs(r[0]);
+          tmem_ld_wait_regs(r[1]);
+          publish(t2_read);
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            float4 d4 = make_float4(row_delta, row_delta, row_delta, row_delta);
+            if constexpr (!kDQ) d4 = *reinterpret_cast<const float4*>(vec + 128 + c);
+            const uint32_t* v = &r[c >> 5][c & 31];
+            const float2 a = __fmul2_rn(make_float2(e[c], e[c + 1]),
+                                        __fadd2_rn(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), make_float2(-d4.x, -d4.y)));
+            const float2 b = __fmul2_rn(make_float2(e[c + 2], e[c + 3]),
+                                        __fadd2_rn(make_float2(__uint_as_float(v[2]), __uint_as_float(v[3])), make_float2(-d4.z, -d4.w)));
+            dw[c >> 1] = pack_bf16x2(a.x, a.y);
+            dw[(c >> 1) + 1] = pack_bf16x2(b.x, b.y);
+          }
+        }
+        // 0 x (NaN - delta): masked places again, on the packed pairs.
+        if (kDQ && i == n - 1 && n * 128 > kv_len) {
+          const int lim = kv_len - i * 128 - wg * 64;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            dw[c] &= (2 * c < lim ? 0xffffu : 0u) | (2 * c + 1 < lim ? 0xffff0000u : 0u);
+          }
+        }
+        if (partial) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) dw[c] = row_ok ? dw[c] : 0u;
+        }
+        tmem_st_32x32b_x32(reg1(g) + half + 32u, dw);
+        tmem_st_wait();
+        publish(ds_ready(g));
       }
-      tmem_st_32x32b_x32(reg1(i) + half + 32u, dw);
-      tmem_st_wait();
-      publish(ds_ready(i));
-    }
-    // ---- gradients out: acc -> bf16 -> TMA store through X1 / X2 ------------------
-    // dQ: warpgroup wg stores columns 64 wg ..; dK/dV: warpgroup 0 dK, 1 dV.
-    if (n > 0 && ok) wait(acc_full, 0u);
-    if (ok) {
-      const float f = kDQ || wg == 0 ? p.scale : 1.0f;
-      const uint32_t acc = (kDQ || wg == 0 ? acc1 : acc2) + lane_off;
-      const CUtensorMap* map = kDQ ? &tm.dq : (wg == 0 ? &tm.dk : &tm.dv);
+      if (!ok) break;
+      // ---- the item's gradients: acc -> bf16 -> global memory, columns 64 wg .. of each ----
+      // (The next item's P or dS of this warp comes after its loads here, so
+      // the accumulators are not overwritten before.)
+      if (n > 0 && !wait(acc_full, filled & 1u)) break;
 #pragma unroll 1
       for (int h = 0; h < (kDQ ? 1 : 2); ++h) {
-        const int col = kDQ ? wg * 64 : h * 64;
-        const uint32_t stage = (wg == 0 ? sX1 : sX2) + (uint32_t)(h * 16384 + qw * 4096);
         uint32_t lo[32], hi[32];
         if (n > 0) {
-          tmem_ld_32x32b_x32(acc + (uint32_t)col, lo);
-          tmem_ld_32x32b_x32(acc + (uint32_t)(col + 32), hi);
+          const uint32_t acc = (h == 0 ? acc1 : acc2) + half;
+          tmem_ld_32x32b_x32(acc, lo);
+          tmem_ld_32x32b_x32(acc + 32u, hi);
           tmem_ld_wait_regs(lo);
           tmem_ld_wait_regs(hi);
         }
+        if (n == 0 || !row_ok) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          lo[c] = n > 0 && row_ok ? __float_as_uint(__uint_as_float(lo[c]) * f) : 0u;
-          hi[c] = n > 0 && row_ok ? __float_as_uint(__uint_as_float(hi[c]) * f) : 0u;
+          for (int c = 0; c < 32; ++c) lo[c] = hi[c] = 0u;
         }
-        stage_row64(lo, hi, false, stage, 0u, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_4d(map, stage, col, head, tile * 128 + qw * 32, bat);
-          bulk_commit_group();
-        }
+        store_grad(kDQ ? p.dq : (h == 0 ? p.dk : p.dv), t.bat, t.tile * 128 + qw * 32, kDQ ? p.q_len : p.kv_len, t.head,
+                   wg * 64, lane, lo, hi, h == 0 ? p.scale : 1.0f);
       }
-      if (lane == 0) bulk_wait_group_read<0>();
-      __syncwarp();
-    } else if (lane == 0) {
-      attn_raise(p, abort_flag, kDevTimeoutEpilogue);
+      tc_fence_before();
+      if (n > 0) {
+        g0 += (uint32_t)n;
+        ++filled;
+      }
     }
+    if (!ok && lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
   }
 
   tc_fence_before();
@@ -508,19 +674,8 @@ __device__ __forceinline__ void attn_bwd_body(const AttnBwdMaps& tm, const AttnB
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
-}
-
-__global__ void __launch_bounds__(kAttnThreads, 1)
-    attn_bwd_kernel(const __grid_constant__ AttnBwdMaps tm, const __grid_constant__ AttnBwdParams p) {
-#if B200_NO_SM100A_FEATURES
-  if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, (uint32_t)kDevWrongArch);
-#else
-  const int cta = (int)blockIdx.x;
-  if (cta < p.dkv_ctas) {
-    attn_bwd_body<false>(tm, p, cta);
-  } else {
-    attn_bwd_body<true>(tm, p, cta - p.dkv_ctas);
-  }
+  // Started early: what follows this kernel must find the dK/dV kernel complete too.
+  if (kDQ && p.early != 0u) pdl_wait();
 #endif  // B200_NO_SM100A_FEATURES
 }
 

@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <utility>
 
 #include "attn_bwd_sm100.cuh"
 #include "attn_sm100.cuh"
@@ -58,11 +59,16 @@ int init_stored(const b200::DeviceInfo& di, StoredState& st) {
   cudaFuncAttributes fa{};
   if (cudaFuncGetAttributes(&fa, b200::flash_attn_fwd_kernel<true>) != cudaSuccess) return B200_ERR_CUDA;
   st.cross_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
-  if (cudaFuncSetAttribute(b200::attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b200::kAttnBwdSmem) !=
-          cudaSuccess ||
-      cudaFuncGetAttributes(&fa, b200::attn_bwd_kernel) != cudaSuccess)
-    return B200_ERR_CUDA;
-  st.bwd_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
+  st.bwd_regs_ok = true;
+  const std::pair<const void*, int> bwd[2] = {
+      {(const void*)b200::attn_bwd_kernel<false>, b200::AttnBwdPlan<false>::kAllocBytes},
+      {(const void*)b200::attn_bwd_kernel<true>, b200::AttnBwdPlan<true>::kAllocBytes}};
+  for (const auto& k : bwd) {
+    if (cudaFuncSetAttribute(k.first, cudaFuncAttributeMaxDynamicSharedMemorySize, k.second) != cudaSuccess ||
+        cudaFuncGetAttributes(&fa, k.first) != cudaSuccess)
+      return B200_ERR_CUDA;
+    if (fa.numRegs != (int)b200::kAttnRegsLaunch) st.bwd_regs_ok = false;
+  }
   for (int f = 0; f < 2; ++f) {
     for (int t = 0; t < 2; ++t) {
       const SplitVariant& v = kSplit[f][t];
@@ -457,8 +463,9 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
 
 namespace {
 int64_t bwd_padded(int64_t q_len) { return (q_len + 127) / 128 * 128; }
+// Two item counters (padded), then lse2 and delta of every padded query row.
 size_t bwd_bytes(int64_t batch, int64_t q_len, int64_t heads) {
-  return 2 * sizeof(float) * (size_t)(batch * heads) * (size_t)bwd_padded(q_len);
+  return kWsAlign + 2 * sizeof(float) * (size_t)(batch * heads) * (size_t)bwd_padded(q_len);
 }
 }  // namespace
 
@@ -484,8 +491,8 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   const bool queries = q_len > 0 && heads > 0, keys = kv_len > 0 && kv_heads > 0;
   if (batch == 0 || (!queries && !keys)) return B200_OK;
   const int64_t q_tiles = queries ? (q_len + 127) / 128 : 0, kv_tiles = keys ? (kv_len + 127) / 128 : 0;
-  const int64_t dkv_ctas = kv_tiles * kv_heads * batch, dq_ctas = q_tiles * heads * batch;
-  if (kv_len > kLim - 128 || q_len > kLim - 128 || dkv_ctas > kLim || dq_ctas > kLim - dkv_ctas ||
+  const int64_t dkv_items = kv_tiles * kv_heads * batch, dq_items = q_tiles * heads * batch;
+  if (kv_len > kLim - 128 || q_len > kLim - 128 || dkv_items > kLim || dq_items > kLim - dkv_items ||
       q_tiles * std::max<int64_t>(heads, 1) > kLim)
     return B200_ERR_TOO_LARGE;
   b200_attn_view qq{}, oo{}, dd{}, dqv{}, kk{}, vv{}, dkv{}, dvv{};
@@ -495,9 +502,9 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
         (rc = check_view(dq, batch, q_len, heads, &dqv)) != B200_OK)
       return rc;
     if (lse == nullptr) return B200_ERR_INVALID_ARG;
-    if (workspace == nullptr || workspace_bytes < bwd_bytes(batch, q_len, heads)) return B200_ERR_INVALID_ARG;
-    if (!aligned(workspace, kWsAlign)) return B200_ERR_ALIGNMENT;
   }
+  if (workspace == nullptr || workspace_bytes < bwd_bytes(batch, q_len, heads)) return B200_ERR_INVALID_ARG;
+  if (!aligned(workspace, kWsAlign)) return B200_ERR_ALIGNMENT;
   if (keys && ((rc = check_view(k, batch, kv_len, kv_heads, &kk)) != B200_OK ||
                (rc = check_view(v, batch, kv_len, kv_heads, &vv)) != B200_OK ||
                (rc = check_view(dk, batch, kv_len, kv_heads, &dkv)) != B200_OK ||
@@ -511,14 +518,14 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   b200::AttnBwdMaps tm{};
   if (queries && ((rc = encode_view(di, &tm.q, qq, batch, q_len, heads, 128, true)) != B200_OK ||
-                  (rc = encode_view(di, &tm.dout, dd, batch, q_len, heads, 128, true)) != B200_OK ||
-                  (rc = encode_view(di, &tm.dq, dqv, batch, q_len, heads, 32, false)) != B200_OK))
+                  (rc = encode_view(di, &tm.dout, dd, batch, q_len, heads, 128, true)) != B200_OK))
     return rc;
   if (keys && ((rc = encode_view(di, &tm.k, kk, batch, kv_len, kv_heads, 128, true)) != B200_OK ||
-               (rc = encode_view(di, &tm.v, vv, batch, kv_len, kv_heads, 128, true)) != B200_OK ||
-               (rc = encode_view(di, &tm.dk, dkv, batch, kv_len, kv_heads, 32, false)) != B200_OK ||
-               (rc = encode_view(di, &tm.dv, dvv, batch, kv_len, kv_heads, 32, false)) != B200_OK))
+               (rc = encode_view(di, &tm.v, vv, batch, kv_len, kv_heads, 128, true)) != B200_OK))
     return rc;
+  // A side that is empty has no map of its own and is not read.
+  if (!queries) tm.q = tm.dout = tm.k;
+  if (!keys) tm.k = tm.v = tm.q;
   b200::AttnBwdParams p{};
   p.q_len = (int32_t)q_len;
   p.kv_len = (int32_t)(keys ? kv_len : 0);
@@ -528,31 +535,48 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   p.batch = (int32_t)batch;
   p.q_tiles = (int32_t)q_tiles;
   p.kv_tiles = (int32_t)kv_tiles;
-  p.dkv_ctas = (int32_t)dkv_ctas;
   p.kv_lens = kv_lens;
   p.scale = scale;
   p.scale_log2 = kLog2e * scale;
   p.timeout_ns = di.timeout_ns;
   p.status = di.status;
-  if (queries) {
-    p.lse2 = static_cast<float*>(workspace);
-    p.delta = p.lse2 + (size_t)(batch * heads) * (size_t)(q_tiles * 128);
-    b200::AttnBwdDeltaParams d{};
-    d.o = static_cast<const __nv_bfloat16*>(oo.data);
-    d.o_batch = oo.batch_stride, d.o_seq = oo.seq_stride, d.o_head = oo.head_stride;
-    d.dout = static_cast<const __nv_bfloat16*>(dd.data);
-    d.d_batch = dd.batch_stride, d.d_seq = dd.seq_stride, d.d_head = dd.head_stride;
-    d.lse = lse;
-    d.lse2 = p.lse2;
-    d.delta = p.delta;
-    d.q_len = p.q_len;
-    d.heads = p.heads;
-    d.padded = (int32_t)(q_tiles * 128);
-    const int64_t rows = batch * heads;
-    d.rows = (int32_t)rows;
-    const dim3 grid((unsigned)(q_tiles * 16), (unsigned)std::min<int64_t>(rows, 65535), (unsigned)((rows + 65534) / 65535));
-    if ((rc = launch(b200::attn_bwd_delta_kernel, grid, 256, 0, stream, d)) != B200_OK) return rc;
+  auto grad = [](const b200_attn_view& g) {
+    return b200::AttnGrad{static_cast<__nv_bfloat16*>(g.data), g.batch_stride, g.seq_stride, g.head_stride};
+  };
+  p.dq = grad(dqv), p.dk = grad(dkv), p.dv = grad(dvv);
+  uint32_t* counters = static_cast<uint32_t*>(workspace);
+  b200::AttnBwdDeltaParams d{};
+  d.o = static_cast<const __nv_bfloat16*>(oo.data);
+  d.o_batch = oo.batch_stride, d.o_seq = oo.seq_stride, d.o_head = oo.head_stride;
+  d.dout = static_cast<const __nv_bfloat16*>(dd.data);
+  d.d_batch = dd.batch_stride, d.d_seq = dd.seq_stride, d.d_head = dd.head_stride;
+  d.lse = lse;
+  d.lse2 = reinterpret_cast<float*>(static_cast<char*>(workspace) + kWsAlign);
+  d.delta = d.lse2 + (size_t)(batch * heads) * (size_t)(q_tiles * 128);
+  d.q_len = p.q_len;
+  d.heads = (int32_t)std::max<int64_t>(heads, 1);
+  d.padded = (int32_t)(q_tiles * 128);
+  d.rows = (int32_t)(batch * heads);
+  d.counters = counters;
+  p.lse2 = d.lse2;
+  p.delta = d.delta;
+  const int64_t rows = std::max<int64_t>(batch * heads, 1);
+  const dim3 grid((unsigned)std::max<int64_t>(q_tiles * 2, 1), (unsigned)std::min<int64_t>(rows, 65535),
+                  (unsigned)((rows + 65534) / 65535));
+  if ((rc = launch(b200::attn_bwd_delta_kernel, grid, 256, 0, stream, d)) != B200_OK) return rc;
+  if (dkv_items > 0) {
+    p.items = (int32_t)dkv_items;
+    p.counter = counters;
+    if ((rc = launch(b200::attn_bwd_kernel<false>, dim3((unsigned)std::min<int64_t>(dkv_items, di.sm_count)),
+                     b200::kAttnThreads, b200::AttnBwdPlan<false>::kAllocBytes, stream, tm, p)) != B200_OK)
+      return rc;
   }
-  return launch(b200::attn_bwd_kernel, dim3((unsigned)(dkv_ctas + dq_ctas)), b200::kAttnThreads, b200::kAttnBwdSmem, stream,
-                tm, p);
+  if (dq_items > 0) {
+    p.items = (int32_t)dq_items;
+    p.counter = counters + 1;
+    p.early = dkv_items > 0 ? 1u : 0u;
+    rc = launch(b200::attn_bwd_kernel<true>, dim3((unsigned)std::min<int64_t>(dq_items, di.sm_count)), b200::kAttnThreads,
+                b200::AttnBwdPlan<true>::kAllocBytes, stream, tm, p);
+  }
+  return rc;
 }

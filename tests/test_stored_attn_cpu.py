@@ -126,7 +126,7 @@ def test_cross_attn_backward_refusals():
     assert call(scale=math.nan) == bad
     assert call(lse=None) == bad
     assert call(ws=None) == bad
-    assert call(n=2 * 4 * 8 * 128 - 1) == bad
+    assert call(n=256 + 2 * 4 * 8 * 128 - 1) == bad
     assert call(q=_view(data=None)) == bad
     assert call(dv=_view(sh=64)) == bad
     assert call(o=_view(data=FAKE + 8)) == _lib.B200_ERR_ALIGNMENT
@@ -137,7 +137,7 @@ def test_cross_attn_backward_refusals():
     assert call(q_len=0, kv_len=0) == _lib.B200_OK
     n = ctypes.c_size_t(0)
     assert lib.b200_cross_attn_bwd_workspace_bytes(2, 129, 4, ctypes.byref(n)) == _lib.B200_OK
-    assert n.value == 2 * 4 * 8 * 256  # two floats per query row, whole tiles
+    assert n.value == 256 + 2 * 4 * 8 * 256  # item counters, and two floats per query row of whole tiles
     assert lib.b200_cross_attn_bwd_workspace_bytes(2, -1, 4, ctypes.byref(n)) == bad
 
 
