@@ -17,7 +17,7 @@
 // Items are handed out by a counter (the delta kernel zeroes it), since their
 // lengths differ; the pipeline runs on from item to item: the next item's tiles load and its first
 // products run while the last one's gradients are stored.  (A CTA per item: 134
-// us against PPAIRS on 8 ragged pairs of 500 queries and up to 1333 keys, 16
+// us against 115 on 8 ragged pairs of 500 queries and up to 1333 keys, 16
 // heads, where an item has 4 to 11 tile pairs and start-up, epilogue and CTA
 // exchange took as long as those.)
 //
@@ -30,8 +30,10 @@
 //
 // 384 threads: warps 0..7 compute, two warpgroups of 64 columns each, one
 // thread per row; warp 8 item fetch and TMA producer, warp 9 MMA issuer and
-// TMEM owner, warps 10, 11 (dQ) zero the K rows past the last key in an item's
-// last tile (they may hold NaN, and 0 x NaN would reach dQ).
+// TMEM owner.  Warps 10, 11 write the gradients of items without tiles (zeros:
+// behind the keys of a padded batch that is much of the memory traffic, and here
+// it runs beside the other items' products) and zero the K rows past the last
+// key in a dQ item's last tile (they may hold NaN, and 0 x NaN would reach dQ).
 // TMEM, 512 columns: a warpgroup puts P and dS over its own half of T1, so no
 // warp waits for another.  dK/dV: T1 and T2 swap two regions from tile to
 // tile, T1 of the next tile being computed while dS of this one is.  dQ: T1
@@ -142,7 +144,9 @@ struct AttnBwdPlan {
   static constexpr int kOffY1 = 2 * kTileBytes;
   static constexpr int kOffY2 = kOffY1 + kY1Stages * kTileBytes;
   static constexpr int kOffVec = kOffY2 + kY2Stages * kTileBytes;  // dK/dV: lse2 and delta of a Y1 stage's rows
-  static constexpr int kOffBar = kOffVec + (kDQ ? 0 : kY1Stages * 1024);
+  // dK/dV: 2 KiB per computing warp for its gradient rows on their way out.
+  static constexpr int kOffOut = kOffVec + (kDQ ? 0 : kY1Stages * 1024);
+  static constexpr int kOffBar = kOffOut + (kDQ ? 0 : 8 * 2048);
   static constexpr int kNumBars = 2 + 3 * kY1Stages + 2 * kY2Stages + 2 + 1 + 1 + 1 + 2 + 1 + 1 + 4;
   static constexpr int kOffItem = kOffBar + kNumBars * 8;  // two slots of (item or -1, keys of its entry)
   static constexpr int kOffTmemHolder = kOffItem + 16;
@@ -152,12 +156,16 @@ struct AttnBwdPlan {
   static_assert(kAllocBytes <= 232448, "attention backward shared memory plan exceeds 227 KiB");
 };
 
-// 32 rows x 64 columns of a gradient, a row per lane in fp32 registers, scaled
-// by f: bf16, transposed within groups of eight lanes (three exchanges), so that eight
-// lanes store one row's 128 bytes.  (Each lane storing its own row, 16 bytes of 32
-// rows at a time, took 1.6 us a tile.)  Rows from `rows` on are not stored.
+// 32 rows x 64 columns of a gradient, a row per lane in fp32 registers, times f,
+// as bf16.  Lanes that store their own rows, 16 bytes of 32 rows at a time, take
+// 1.6 us a tile, so the lanes exchange first and then store whole rows: dK/dV
+// through 2 KiB of shared memory per warp, 32 columns at a time (four lanes per
+// row); dQ, whose third K stage leaves no room for that, by three exchanges
+// within groups of eight lanes (eight lanes per row; 1.1 us).  Rows from `rows` on are
+// not stored.
+template <bool kDQ>
 __device__ __forceinline__ void store_grad(const AttnGrad& g, int bat, int row0, int rows, int head, int col, uint32_t lane,
-                                           const uint32_t (&lo)[32], const uint32_t (&hi)[32], float f) {
+                                           const uint32_t (&lo)[32], const uint32_t (&hi)[32], float f, uint32_t buf) {
   uint32_t w[8][4];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -165,28 +173,65 @@ __device__ __forceinline__ void store_grad(const AttnGrad& g, int bat, int row0,
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[j][k] = pack_bf16x2(__uint_as_float(v[2 * k]) * f, __uint_as_float(v[2 * k + 1]) * f);
   }
+  __nv_bfloat16* dst = g.data + bat * g.batch_stride + head * g.head_stride + col;
+  if constexpr (!kDQ) {
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) {
-    const bool upper = (lane & (uint32_t)d) != 0;
+    for (int h = 0; h < 2; ++h) {
+      // 64 bytes a row; the 16-byte cells are permuted so that both directions touch every bank once.
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j & d) continue;
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = buf + lane * 64u + (((uint32_t)j ^ ((lane >> 1) & 3u)) << 4);
+        const uint32_t* v = w[4 * h + j];
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+      }
+      __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[j][k] : w[j | d][k], d);
-        if (upper) {
-          w[j][k] = got;
-        } else {
-          w[j | d][k] = got;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t r = (uint32_t)(8 * i) + (lane >> 2), c = lane & 3u;
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(buf + r * 64u + ((c ^ ((r >> 1) & 3u)) << 4))
+                     : "memory");
+        const int row = row0 + (int)r;
+        if (row < rows) *reinterpret_cast<uint4*>(dst + row * g.seq_stride + 32 * h + 8 * (int)c) = v;
+      }
+      __syncwarp();
+    }
+  } else {
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+      const bool upper = (lane & (uint32_t)d) != 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j & d) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[j][k] : w[j | d][k], d);
+          if (upper) {
+            w[j][k] = got;
+          } else {
+            w[j | d][k] = got;
+          }
         }
       }
     }
-  }
-  const int first = row0 + (int)(lane & 24u);
-  __nv_bfloat16* dst = g.data + bat * g.batch_stride + first * g.seq_stride + head * g.head_stride + col + 8 * (lane & 7u);
+    const int first = row0 + (int)(lane & 24u);
+    dst += first * g.seq_stride + 8 * (lane & 7u);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (first + j < rows) *reinterpret_cast<uint4*>(dst + j * g.seq_stride) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+    for (int j = 0; j < 8; ++j) {
+      if (first + j < rows) *reinterpret_cast<uint4*>(dst + j * g.seq_stride) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+    }
+  }
+}
+
+// The same of zeros.
+__device__ __forceinline__ void store_zeros(const AttnGrad& g, int bat, int row0, int rows, int head, int col, uint32_t lane) {
+  const int first = row0 + (int)(lane >> 3);
+  __nv_bfloat16* dst = g.data + bat * g.batch_stride + head * g.head_stride + first * g.seq_stride + col + 8 * (lane & 7u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (first + 4 * i < rows) *reinterpret_cast<uint4*>(dst + 4 * i * g.seq_stride) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -198,7 +243,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #else
   using Plan = AttnBwdPlan<kDQ>;
   constexpr int S1 = Plan::kY1Stages, S2 = Plan::kY2Stages;
-  constexpr int kReaders = kDQ ? 11 : 9;  // of an item: MMA issuer, 8 computing warps, dQ: the two cleaning warps
+  constexpr int kReaders = 11;  // of an item: MMA issuer, 8 computing warps, warps 10 and 11
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base = (raw_u32 + 1023u) & ~1023u;
@@ -281,6 +326,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   pdl_launch_dependents();
 
   // An item: its tile, head and entry, and the number of tiles to stream.
+  // Tiles change fastest: neighbours stream the same tiles.  (Entries fastest, so
+  // that long and short ones alternate: 4 % slower on 8 ragged pairs.)
   struct Item {
     int tile, head, bat, kv_len, n;
     bool clean;  // dQ: rows of the last K tile past the last key, which TMA filled from memory
@@ -487,8 +534,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (!mbar_wait(drain, 0u, p.timeout_ns, nullptr)) attn_raise(p, abort_flag, kDevTimeoutDrain);
       }
       __syncwarp();
-    } else if (kDQ) {
-      // ---- warps 10, 11: zero the K rows past an item's last key ----------------
+    } else {
+      // ---- warps 10, 11: gradients that are zero; K rows past an item's last key ----
       // Every decision is made by both warps together (a barrier that also
       // carries it), so that neither waits for the other at a later one.
       auto both = [&](bool mine) { return named_bar_and(1, 64, __all_sync(0xffffffffu, mine)); };
@@ -502,8 +549,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (lane == 0) mbar_arrive(item_empty(k));
         if (id < 0) break;
         const Item t = item_of(id, kv_len);
+        if (t.n == 0) {
+#pragma unroll 1
+          for (int part = warp - kAttnMmaWarp - 1; part < 8; part += 2) {  // 32 rows x 64 columns
+            const int row0 = t.tile * 128 + (part >> 1) * 32, rows = kDQ ? p.q_len : p.kv_len, col = (part & 1) * 64;
+            store_zeros(kDQ ? p.dq : p.dk, t.bat, row0, rows, t.head, col, lane);
+            if constexpr (!kDQ) store_zeros(p.dv, t.bat, row0, rows, t.head, col, lane);
+          }
+          continue;
+        }
         g += (uint32_t)t.n;
-        if (!t.clean || t.n == 0) continue;
+        if (!t.clean) continue;
         const uint32_t last = g - 1;
         ok = both(mbar_wait(y1_raw(last), (raw_par >> (last % S1)) & 1u, p.timeout_ns, abort_flag));
         if (!ok) break;
@@ -543,6 +599,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     Item t;
     for (uint32_t k = 0; ok && next_item(k, true, &t, &ok); ++k) {
       const int kv_len = t.kv_len, n = t.n;
+      if (n == 0) continue;
       float row_lse = 0.0f, row_delta = 0.0f;  // dQ: of this thread's query row
       if constexpr (kDQ) {
         const size_t at = ((size_t)t.bat * p.heads + t.head) * (size_t)(p.q_tiles * 128) + t.tile * 128 + row;
@@ -641,29 +698,27 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // ---- the item's gradients: acc -> bf16 -> global memory, columns 64 wg .. of each ----
       // (The next item's P or dS of this warp comes after its loads here, so
       // the accumulators are not overwritten before.)
-      if (n > 0 && !wait(acc_full, filled & 1u)) break;
+      if (!wait(acc_full, filled & 1u)) break;
+      const int rows = kDQ ? p.q_len : p.kv_len;
 #pragma unroll 1
       for (int h = 0; h < (kDQ ? 1 : 2); ++h) {
+        const AttnGrad& grad = kDQ ? p.dq : (h == 0 ? p.dk : p.dv);
         uint32_t lo[32], hi[32];
-        if (n > 0) {
-          const uint32_t acc = (h == 0 ? acc1 : acc2) + half;
-          tmem_ld_32x32b_x32(acc, lo);
-          tmem_ld_32x32b_x32(acc + 32u, hi);
-          tmem_ld_wait_regs(lo);
-          tmem_ld_wait_regs(hi);
-        }
-        if (n == 0 || !row_ok) {
+        const uint32_t acc = (h == 0 ? acc1 : acc2) + half;
+        tmem_ld_32x32b_x32(acc, lo);
+        tmem_ld_32x32b_x32(acc + 32u, hi);
+        tmem_ld_wait_regs(lo);
+        tmem_ld_wait_regs(hi);
+        if (!row_ok) {
 #pragma unroll
           for (int c = 0; c < 32; ++c) lo[c] = hi[c] = 0u;
         }
-        store_grad(kDQ ? p.dq : (h == 0 ? p.dk : p.dv), t.bat, t.tile * 128 + qw * 32, kDQ ? p.q_len : p.kv_len, t.head,
-                   wg * 64, lane, lo, hi, h == 0 ? p.scale : 1.0f);
+        store_grad<kDQ>(grad, t.bat, t.tile * 128 + qw * 32, rows, t.head, wg * 64, lane, lo, hi, h == 0 ? p.scale : 1.0f,
+                        base + (uint32_t)(Plan::kOffOut + warp * 2048));
       }
       tc_fence_before();
-      if (n > 0) {
-        g0 += (uint32_t)n;
-        ++filled;
-      }
+      g0 += (uint32_t)n;
+      ++filled;
     }
     if (!ok && lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
   }
