@@ -45,7 +45,9 @@
 // or past it are -inf; their V rows may hold anything (NaN included), and
 // 0 x NaN would reach O through the product, so the two idle warps zero those
 // rows of the last V tile in shared memory before its product; a batch entry
-// without keys writes O = 0 and lse = -inf.
+// without keys writes O = 0 and lse = -inf.  A grid that would leave SMs idle is
+// split along the keys (gridDim.z): each part writes its own normalised O in
+// fp32 and its lse, and attn_merge_kernel (attn_split_sm100.cuh) adds the parts.
 #pragma once
 
 #include <cuda.h>
@@ -109,7 +111,8 @@ struct AttnParams {
   // Cross attention only.
   int32_t kv_len;          // rows of K and V
   const int32_t* kv_lens;  // [batch] keys of each batch entry (clamped to [0, kv_len]), or NULL: kv_len
-  float* lse;              // [batch, heads, seq_len] natural log of the softmax denominator, or NULL
+  float* lse;              // [batch, heads, seq_len] natural log of the softmax denominator, or NULL;
+                           // with several parts: of each, [gridDim.z, batch, heads, seq_len]
 };
 
 struct AttnSmemPlan {
@@ -214,6 +217,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     flash_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                           const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
                           const __grid_constant__ AttnParams p) {
+  // (Cross attention in parts: tmO is the fp32 map of their O, {128, seq_len, parts x batch x heads}.)
 #if B200_NO_SM100A_FEATURES
   if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, (uint32_t)kDevWrongArch);
 #else
@@ -254,7 +258,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     qt_of[1] = p.num_q_tiles - 1 - (int)blockIdx.y;
     if (qt_of[1] <= qt_of[0]) qt_of[1] = p.num_q_tiles;  // the middle tile of an odd count stays alone
   } else {
-    qt_of[0] = kAttnQTiles * ((int)gridDim.y - 1 - (int)blockIdx.y);
+    // (Without a causal mask the last CTA row is the shorter one, if any.)
+    qt_of[0] = kAttnQTiles * (kCross ? (int)blockIdx.y : (int)gridDim.y - 1 - (int)blockIdx.y);
     qt_of[1] = qt_of[0] + 1;
   }
   const int head = (int)blockIdx.x % p.heads;
@@ -306,12 +311,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto kv_tiles = [&](int qt) {
     return qt >= p.num_q_tiles ? 0 : (p.causal ? min(qt + 1, kv_tiles_all) : kv_tiles_all);
   };
-  const int n0 = kv_tiles(qt_of[0]);
-  const int n1 = kv_tiles(qt_of[1]);  // >= n0, or 0
+  int n0 = kv_tiles(qt_of[0]);
+  int n1 = kv_tiles(qt_of[1]);  // >= n0, or 0
+  [[maybe_unused]] int first = 0;  // first key tile of this part
+  // Rows of the last V tile past the last key, which TMA filled from memory.
+  bool clean_v = kCross && kv_len < p.kv_len && kv_len % kAttnBKV != 0;
+  if constexpr (kCross) {
+    if (gridDim.z > 1) {
+      const int parts = (int)gridDim.z, z = (int)blockIdx.z;
+      first = (int)((int64_t)kv_tiles_all * z / parts);
+      const int n = (int)((int64_t)kv_tiles_all * (z + 1) / parts) - first;
+      clean_v = clean_v && n > 0 && first + n == kv_tiles_all;
+      kv_len -= first * kAttnBKV;  // keys from this part's first tile on
+      n0 = n0 > 0 ? n : 0;
+      n1 = n1 > 0 ? n : 0;
+    }
+  }
   const int n_max = max(n0, n1);
   const int n_q = n1 > 0 ? 2 : (n0 > 0 ? 1 : 0);  // query tiles this CTA reads
-  // Rows of the last V tile past the last key, which TMA filled from memory.
-  const bool clean_v = kCross && kv_len < p.kv_len && kv_len % kAttnBKV != 0;
 
   if (warp >= kAttnProducerWarp) {
     setmaxnreg_dec<kAttnRegsOther>();
@@ -343,8 +360,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           mbar_arrive_expect_tx(k_full(sk), Plan::kTileBytes);
           for (int h = 0; h < 2; ++h) {
             if constexpr (kCross) {
-              tma_load_4d(sK + sk * Plan::kTileBytes + h * 16384, &tmK, k_full(sk), 64 * h, kv_head, j * kAttnBKV, bat,
-                          pol_keep);
+              tma_load_4d(sK + sk * Plan::kTileBytes + h * 16384, &tmK, k_full(sk), 64 * h, kv_head, (first + j) * kAttnBKV,
+                          bat, pol_keep);
             } else {
               tma_load_3d(sK + sk * Plan::kTileBytes + h * 16384, &tmK, k_full(sk), kv_col0 + 64 * h, j * kAttnBKV,
                           bat, pol_keep);
@@ -365,7 +382,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             for (int h = 0; h < 2; ++h) {
               const uint32_t dst = sV + sv * Plan::kTileBytes + hk * 16384 + h * 8192;
               if constexpr (kCross) {
-                tma_load_4d(dst, &tmV, v_bar, 64 * h, kv_head, j * kAttnBKV + 64 * hk, bat, pol_keep);
+                tma_load_4d(dst, &tmV, v_bar, 64 * h, kv_head, (first + j) * kAttnBKV + 64 * hk, bat, pol_keep);
               } else {
                 tma_load_3d(dst, &tmV, v_bar, kv_col0 + 64 * h, j * kAttnBKV + 64 * hk, bat, pol_keep);
               }
@@ -606,7 +623,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
         if constexpr (kCross) {
           if (p.lse != nullptr && q_idx < p.seq_len) {
-            p.lse[((size_t)bat * p.heads + head) * p.seq_len + q_idx] =
+            p.lse[(((size_t)blockIdx.z * p.batch + bat) * p.heads + head) * p.seq_len + q_idx] =
                 l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
         }
@@ -623,11 +640,28 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             lo[i] = __float_as_uint(__uint_as_float(lo[i]) * inv_l);
             hi[i] = __float_as_uint(__uint_as_float(hi[i]) * inv_l);
           }
+          if constexpr (kCross) {
+            if (gridDim.z > 1) {
+              // Two boxes of 32 fp32 columns: the whole 8 KiB of this warp, twice.
+              stage_row64(lo, hi, true, stage, stage + 4096u, lane);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                const int part_row = ((int)blockIdx.z * p.batch + bat) * p.heads + head;
+                tma_store_3d(&tmO, stage, 64 * half, qt * kAttnBQ + qw * 32, part_row);
+                tma_store_3d(&tmO, stage + 4096u, 64 * half + 32, qt * kAttnBQ + qw * 32, part_row);
+                bulk_commit_group();
+                bulk_wait_group_read<0>();
+              }
+              __syncwarp();
+              continue;
+            }
+          }
           stage_row64(lo, hi, false, stage + (uint32_t)(half * 4096), 0u, lane);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
+        if (lane == 0 && !(kCross && gridDim.z > 1)) {
           for (int half = 0; half < 2; ++half) {
             if constexpr (kCross) {
               tma_store_4d(&tmO, stage + (uint32_t)(half * 4096), 64 * half, head, qt * kAttnBQ + qw * 32, bat);
@@ -643,18 +677,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         attn_raise(p, abort_flag, kDevTimeoutEpilogue);
       }
     } else if (kCross && qt < p.num_q_tiles) {
-      // No keys: O = 0, lse = -inf.  (Q was not loaded: its buffer stages the zeros.)
+      // No keys: O = 0, lse = -inf.  (Q was not loaded: its buffer stages the
+      // zeros.  Of a part only the lse counts.)
       const uint32_t stage = sQ + (uint32_t)(tile * Plan::kTileBytes + qw * 8192);
       uint32_t zero[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) zero[i] = 0u;
       stage_row64(zero, zero, false, stage, 0u, lane);
       if (p.lse != nullptr && q_idx < p.seq_len) {
-        p.lse[((size_t)bat * p.heads + head) * p.seq_len + q_idx] = -INFINITY;
+        p.lse[(((size_t)blockIdx.z * p.batch + bat) * p.heads + head) * p.seq_len + q_idx] = -INFINITY;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && gridDim.z == 1) {
         for (int half = 0; half < 2; ++half) {
           tma_store_4d(&tmO, stage, 64 * half, head, qt * kAttnBQ + qw * 32, bat);
         }

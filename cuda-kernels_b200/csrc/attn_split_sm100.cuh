@@ -903,4 +903,52 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(const __grid
   }
 }
 
+// Adds the parts of cross attention split along the keys: a warp per query
+// row, 4 columns per lane, eight parts in flight, in order.
+struct AttnMergeParams {
+  const float* part_o;    // [parts, batch, heads, q_len, 128]
+  const float* part_lse;  // [parts, batch, heads, q_len]
+  __nv_bfloat16* o;       // [batch, q_len, heads, 128], strides in elements
+  int64_t o_batch, o_seq, o_head;
+  float* lse;             // [batch, heads, q_len] or NULL
+  int32_t parts, heads, q_len;
+  int64_t rows;           // batch * heads * q_len
+};
+__global__ void __launch_bounds__(256) attn_merge_kernel(const __grid_constant__ AttnMergeParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = (int)(threadIdx.x & 31u);
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  float top = -INFINITY;
+  for (int s = lane; s < p.parts; s += 32) top = fmaxf(top, p.part_lse[s * p.rows + row]);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+  float sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s0 = 0; s0 < p.parts; s0 += 8) {
+    float l[8];
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t s = min(s0 + i, p.parts - 1);
+      l[i] = p.part_lse[s * p.rows + row];
+      v[i] = *reinterpret_cast<const float4*>(p.part_o + (s * p.rows + row) * kAttnD + 4 * lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (s0 + i >= p.parts || l[i] == -INFINITY) continue;  // (O of a part without keys is not written)
+      const float w = __expf(l[i] - top);
+      sum += w;
+      acc.x += w * v[i].x, acc.y += w * v[i].y, acc.z += w * v[i].z, acc.w += w * v[i].w;
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t bh = row / p.q_len;
+  const int64_t tok = row - bh * p.q_len;
+  *reinterpret_cast<uint2*>(p.o + bh / p.heads * p.o_batch + tok * p.o_seq + bh % p.heads * p.o_head + 4 * lane) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (p.lse != nullptr && lane == 0) p.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
+}
+
 }  // namespace b200

@@ -22,33 +22,29 @@ constexpr int kMaxDevices = 64;
 constexpr int64_t kLim = 0x7fffffffLL;
 constexpr size_t kWsAlign = 256;
 
-// Cross attention: at most this many query rows per key/value head run split
-// along the keys (attn_split_kernel), more on the tcgen05 kernel.
-constexpr int64_t kSplitMaxRows = 64;
-
 using SplitKernel = void (*)(const CUtensorMap, const CUtensorMap, const b200::SplitAttnParams);
 struct SplitVariant {
   SplitKernel kernel;
   void (*join)(const b200::SplitAttnParams);
+  int tiles;  // row tiles per warp
   int smem;
   size_t part_floats;
 };
-// [source: bf16, fp8][row tiles per warp - 1]
-const SplitVariant kSplit[2][2] = {
-    {{b200::attn_split_kernel<false, 1>, b200::attn_join_kernel<1>, b200::SplitPlan<false, 1>::kAllocBytes,
-      b200::SplitPlan<false, 1>::kPartFloats},
-     {b200::attn_split_kernel<false, 2>, b200::attn_join_kernel<2>, b200::SplitPlan<false, 2>::kAllocBytes,
-      b200::SplitPlan<false, 2>::kPartFloats}},
-    {{b200::attn_split_kernel<true, 1>, b200::attn_join_kernel<1>, b200::SplitPlan<true, 1>::kAllocBytes,
-      b200::SplitPlan<true, 1>::kPartFloats},
-     {b200::attn_split_kernel<true, 2>, b200::attn_join_kernel<2>, b200::SplitPlan<true, 2>::kAllocBytes,
-      b200::SplitPlan<true, 2>::kPartFloats}}};
+// bf16 states of few query rows; the 8-bit cache with one or two row tiles per warp.
+enum SplitIndex { kSplitBf16 = 0, kSplitFp8 = 1, kSplitFp8Wide = 2, kSplitVariants = 3 };
+const SplitVariant kSplit[kSplitVariants] = {
+    {b200::attn_split_kernel<false, 1>, b200::attn_join_kernel<1>, 1, b200::SplitPlan<false, 1>::kAllocBytes,
+     b200::SplitPlan<false, 1>::kPartFloats},
+    {b200::attn_split_kernel<true, 1>, b200::attn_join_kernel<1>, 1, b200::SplitPlan<true, 1>::kAllocBytes,
+     b200::SplitPlan<true, 1>::kPartFloats},
+    {b200::attn_split_kernel<true, 2>, b200::attn_join_kernel<2>, 2, b200::SplitPlan<true, 2>::kAllocBytes,
+     b200::SplitPlan<true, 2>::kPartFloats}};
 
 struct StoredState {
   std::once_flag once;
   int init_rc = B200_OK;
   bool cross_regs_ok = false, bwd_regs_ok = false;  // setmaxnreg shares match the binary (attn_sm100.cuh)
-  int split_ctas[2][2] = {};   // resident CTAs of each split variant on the whole GPU
+  int split_ctas[kSplitVariants] = {};  // resident CTAs of each split variant on the whole GPU
 };
 StoredState g_stored[kMaxDevices];
 
@@ -69,16 +65,14 @@ int init_stored(const b200::DeviceInfo& di, StoredState& st) {
       return B200_ERR_CUDA;
     if (fa.numRegs != (int)b200::kAttnRegsLaunch) st.bwd_regs_ok = false;
   }
-  for (int f = 0; f < 2; ++f) {
-    for (int t = 0; t < 2; ++t) {
-      const SplitVariant& v = kSplit[f][t];
-      int per_sm = 0;
-      if (cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess ||
-          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.kernel, b200::kSplitThreads, v.smem) != cudaSuccess ||
-          per_sm < 1)
-        return B200_ERR_CUDA;
-      st.split_ctas[f][t] = per_sm * di.sm_count;
-    }
+  for (int i = 0; i < kSplitVariants; ++i) {
+    const SplitVariant& v = kSplit[i];
+    int per_sm = 0;
+    if (cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.kernel, b200::kSplitThreads, v.smem) != cudaSuccess ||
+        per_sm < 1)
+      return B200_ERR_CUDA;
+    st.split_ctas[i] = per_sm * di.sm_count;
   }
   return B200_OK;
 }
@@ -140,6 +134,18 @@ int encode_cache(const b200::DeviceInfo& di, CUtensorMap* map, void* codes, int6
   return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
 }
 
+// fp32 parts of cross attention's O, [parts x batch x heads, q_len, 128]: boxes of 32 columns x 32 rows.
+int encode_parts(const b200::DeviceInfo& di, CUtensorMap* map, float* data, int64_t q_len, int64_t outer) {
+  cuuint64_t dims[3] = {(cuuint64_t)b200::kAttnD, (cuuint64_t)q_len, (cuuint64_t)outer};
+  cuuint64_t strides[2] = {(cuuint64_t)b200::kAttnD * 4, (cuuint64_t)b200::kAttnD * 4 * (cuuint64_t)q_len};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = di.encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, data, dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
+}
+
 template <typename... Params, typename... Args>
 int launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -185,66 +191,120 @@ int check_cache_pointers(const b200_kv_cache* c) {
   return B200_OK;
 }
 
-// Launch shape of the split kernel for a problem: fp8 or bf16 source, `rows`
-// query rows per key/value head.
-struct SplitPlanHost {
-  int variant;  // row tiles per warp - 1
+// Launch shape of a split variant for `rows` query rows per key/value head.
+struct SplitShape {
+  SplitIndex index;
   int64_t row_tiles;
   int ctas;
   bool cut;  // some segment can be longer than a unit: partial results need the workspace
   size_t bytes;
 };
-int plan_split_attn(const StoredState& st, bool fp8, int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_len,
-                    SplitPlanHost* out) {
-  out->variant = rows <= 16 ? 0 : 1;
-  const int64_t tile = 16 * (out->variant + 1);
-  out->row_tiles = (rows + tile - 1) / tile;
-  const int64_t keys = fp8 ? b200::SplitPlan<true, 1>::kKeys : b200::SplitPlan<false, 1>::kKeys;
-  const int64_t units = (kv_len + keys - 1) / keys;  // of the longest segment
+int plan_split(const StoredState& st, SplitIndex index, int64_t batch, int64_t rows, int64_t kv_heads, int64_t kv_len,
+               SplitShape* out) {
+  const SplitVariant& v = kSplit[index];
+  out->index = index;
+  out->row_tiles = (rows + 16 * v.tiles - 1) / (16 * v.tiles);
+  constexpr int64_t keys = b200::SplitPlan<true, 1>::kKeys;  // of a unit, the same for all variants
+  const int64_t units = (kv_len + keys - 1) / keys;          // of the longest segment
   const int64_t segs = kv_heads * out->row_tiles;
   if (segs > kLim) return B200_ERR_TOO_LARGE;
-  const int64_t resident = st.split_ctas[fp8 ? 1 : 0][out->variant];
   // One worker per unit at most (in double: the product may pass 2^63).
   const double most = (double)batch * (double)segs * (double)std::max<int64_t>(units, 1);
-  out->ctas = (int)std::min((double)resident, std::ceil(most / b200::kSplitWarps));
+  out->ctas = (int)std::min((double)st.split_ctas[index], std::ceil(most / b200::kSplitWarps));
   out->cut = units > 1;
-  out->bytes = out->cut ? (size_t)(out->ctas * b200::kSplitWarps) * (2 * kSplit[fp8 ? 1 : 0][out->variant].part_floats * sizeof(float) +
-                                               sizeof(int4))
-                        : 0;
+  out->bytes = out->cut ? (size_t)(out->ctas * b200::kSplitWarps) * (2 * v.part_floats * sizeof(float) + sizeof(int4)) : 0;
   out->bytes = (out->bytes + kWsAlign - 1) / kWsAlign * kWsAlign;
   return B200_OK;
 }
 
-int run_split(const b200::DeviceInfo& di, const SplitPlanHost& plan, bool fp8, const CUtensorMap& tmK,
-              const CUtensorMap& tmV, b200::SplitAttnParams& p, void* workspace, size_t workspace_bytes,
-              cudaStream_t stream) {
-  const SplitVariant& v = kSplit[fp8 ? 1 : 0][plan.variant];
-  const int workers = plan.ctas * b200::kSplitWarps;
-  if (plan.bytes > 0) {
-    if (workspace == nullptr || workspace_bytes < plan.bytes) return B200_ERR_INVALID_ARG;
-    if (!aligned(workspace, kWsAlign)) return B200_ERR_ALIGNMENT;
+int check_workspace(const void* workspace, size_t have, size_t need) {
+  if (need == 0) return B200_OK;
+  if (workspace == nullptr || have < need) return B200_ERR_INVALID_ARG;
+  return aligned(workspace, kWsAlign) ? B200_OK : B200_ERR_ALIGNMENT;
+}
+
+int run_split(const b200::DeviceInfo& di, const SplitShape& shape, const CUtensorMap& tmK, const CUtensorMap& tmV,
+              b200::SplitAttnParams& p, void* workspace, cudaStream_t stream) {
+  const SplitVariant& v = kSplit[shape.index];
+  const int workers = shape.ctas * b200::kSplitWarps;
+  if (shape.bytes > 0) {
     p.part = static_cast<float*>(workspace);
     p.desc = reinterpret_cast<int4*>(p.part + 2 * (size_t)workers * v.part_floats);
   }
-  p.row_tiles = (int32_t)plan.row_tiles;
+  p.row_tiles = (int32_t)shape.row_tiles;
   p.workers = workers;
   p.timeout_ns = di.timeout_ns;
   p.status = di.status;
-  const int rc = launch(v.kernel, dim3((unsigned)plan.ctas), b200::kSplitThreads, v.smem, stream, tmK, tmV, p);
-  if (rc != B200_OK || !plan.cut) return rc;
-  const int rows = std::min<int>(p.rows, 16 * (plan.variant + 1));
+  const int rc = launch(v.kernel, dim3((unsigned)shape.ctas), b200::kSplitThreads, v.smem, stream, tmK, tmV, p);
+  if (rc != B200_OK || !shape.cut) return rc;
+  const int rows = std::min<int>(p.rows, 16 * v.tiles);
   const dim3 grid((unsigned)((workers + b200::kJoinWorkers - 1) / b200::kJoinWorkers),
                   (unsigned)std::min(rows, b200::kJoinRowBlocks));
   return launch(v.join, grid, 32 * b200::kJoinWarps, 0, stream, p);
 }
 
+// How cross attention runs: on the split kernel, or on the tcgen05 kernel in
+// `parts` along the keys.
+struct CrossShape {
+  bool few;
+  SplitShape split;
+  int parts;
+  size_t bytes;
+};
+int plan_cross(const b200::DeviceInfo& di, const StoredState& st, int64_t batch, int64_t q_len, int64_t kv_len,
+               int64_t heads, int64_t kv_heads, CrossShape* out) {
+  *out = CrossShape{};
+  out->parts = 1;
+  const int64_t q_tiles = (q_len + b200::kAttnBQ - 1) / b200::kAttnBQ;
+  const int64_t ctas = heads * batch * ((q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles);
+  const int64_t tiles = (kv_len + b200::kAttnBKV - 1) / b200::kAttnBKV;
+  // On a B200 a query tile takes 1.6 us per key tile alone and two together 1.95,
+  // besides 5.5 us to start and end.  While parts fit beside each other (of two
+  // key tiles at least) they save tiles, but cost 4 us for the merge and their
+  // O once out and once back, 1 KiB a row and part at 4 TB/s.  Measured: 128 queries, 4
+  // heads, 4000 keys: 16 parts 13 us against one 56; 256 queries, 2 x 32 heads,
+  // 1000 keys: 2 parts 26 against 21.
+  const int64_t rows = batch * heads * q_len;
+  const double per_tile = q_tiles == 1 ? 1.6 : 1.95;
+  const double waves = std::ceil((double)ctas / di.sm_count);
+  double tc = 5.5 + waves * (double)tiles * per_tile;
+  const int64_t most = ctas < di.sm_count ? std::min(di.sm_count / ctas, tiles / 2) : 1;
+  for (int64_t n = 2; n <= most; ++n) {
+    const double t = 9.5 + (double)((tiles + n - 1) / n) * per_tile + 1024.0 * (double)(rows * n) / 4e6;
+    if (t < tc) {
+      tc = t;
+      out->parts = (int)n;
+    }
+  }
+  // The split kernel reads K and V once, at 5.6 TB/s, besides 9.5 us.  It takes up
+  // to 16 rows per key/value head (with two row tiles per warp it lost to the
+  // tcgen05 kernel in parts: 32 rows, 4 heads, 1000 keys 17 against 11 us).  Measured:
+  // one query, 4 heads: 9.9 against 7.0 us (tcgen05) at 200 keys, 10.4 against 16.8 at
+  // 1000 (one part); 8 x 16 heads, 4000 keys: 52 against 58.
+  if (q_len * (heads / kv_heads) <= 16) {
+    const double split = 9.5 + 4.0 * b200::kKvD * (double)batch * (double)kv_heads * (double)kv_len / 5.6e6;
+    out->few = split < tc;
+  }
+  if (out->few) {
+    out->parts = 1;
+    const int rc = plan_split(st, kSplitBf16, batch, q_len * (heads / kv_heads), kv_heads, kv_len, &out->split);
+    out->bytes = out->split.bytes;
+    return rc;
+  }
+  if (out->parts > 1) out->bytes = (size_t)out->parts * (size_t)(batch * heads * q_len) * (b200::kAttnD + 1) * sizeof(float);
+  out->bytes = (out->bytes + kWsAlign - 1) / kWsAlign * kWsAlign;
+  return B200_OK;
+}
+
+// Over the cache: two row tiles per warp from 17 rows per key/value head on.
+int plan_cache(const StoredState& st, int64_t batch, int64_t rows, const b200_kv_cache* cache, SplitShape* out) {
+  return plan_split(st, rows <= 16 ? kSplitFp8 : kSplitFp8Wide, batch, rows, cache->kv_heads,
+                    cache->max_pages * cache->page_size, out);
+}
+
 bool scale_ok(float scale) { return scale > 0.0f && std::isfinite(scale); }
 
 constexpr float kLog2e = 1.4426950408889634f;
-
-bool cross_splits(int64_t q_len, int64_t heads, int64_t kv_heads) {
-  return kv_heads > 0 && q_len * (heads / kv_heads) <= kSplitMaxRows;
-}
 
 }  // namespace
 
@@ -308,11 +368,9 @@ extern "C" B200_API int b200_cache_attn_workspace_bytes(int64_t batch, int64_t q
   b200::DeviceInfo di;
   StoredState* st = nullptr;
   if ((rc = current_state(&di, &st)) != B200_OK) return rc;
-  SplitPlanHost plan;
-  if ((rc = plan_split_attn(*st, true, batch, q_len * (heads / cache->kv_heads), cache->kv_heads,
-                            cache->max_pages * cache->page_size, &plan)) != B200_OK)
-    return rc;
-  *bytes = plan.bytes;
+  SplitShape shape;
+  if ((rc = plan_cache(*st, batch, q_len * (heads / cache->kv_heads), cache, &shape)) != B200_OK) return rc;
+  *bytes = shape.bytes;
   return B200_OK;
 }
 
@@ -354,8 +412,9 @@ extern "C" B200_API int b200_cache_attn(const b200_attn_view* q, const b200_kv_c
   p.table_stride = cache->table_stride;
   p.k_scale = cache->k_scale;
   p.v_scale = cache->v_scale;
-  SplitPlanHost plan;
-  if ((rc = plan_split_attn(*st, true, batch, p.rows, p.kv_heads, cache->max_pages * cache->page_size, &plan)) != B200_OK)
+  SplitShape shape;
+  if ((rc = plan_cache(*st, batch, p.rows, cache, &shape)) != B200_OK ||
+      (rc = check_workspace(workspace, workspace_bytes, shape.bytes)) != B200_OK)
     return rc;
   CUtensorMap tmK{}, tmV{};
   if (p.kv_len > 0) {
@@ -364,7 +423,7 @@ extern "C" B200_API int b200_cache_attn(const b200_attn_view* q, const b200_kv_c
         (rc = encode_cache(di, &tmV, cache->v, rows, cache->page_size)) != B200_OK)
       return rc;
   }
-  return run_split(di, plan, true, tmK, tmV, p, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream_));
+  return run_split(di, shape, tmK, tmV, p, workspace, reinterpret_cast<cudaStream_t>(stream_));
 }
 
 extern "C" B200_API int b200_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
@@ -375,13 +434,13 @@ extern "C" B200_API int b200_cross_attn_workspace_bytes(int64_t batch, int64_t q
   if (rc != B200_OK) return rc;
   if (kv_len < 0) return B200_ERR_INVALID_ARG;
   if (kv_len > kLim) return B200_ERR_TOO_LARGE;
-  if (batch == 0 || q_len == 0 || heads == 0 || !cross_splits(q_len, heads, kv_heads)) return B200_OK;
+  if (batch == 0 || q_len == 0 || heads == 0) return B200_OK;
   b200::DeviceInfo di;
   StoredState* st = nullptr;
   if ((rc = current_state(&di, &st)) != B200_OK) return rc;
-  SplitPlanHost plan;
-  if ((rc = plan_split_attn(*st, false, batch, q_len * (heads / kv_heads), kv_heads, kv_len, &plan)) != B200_OK) return rc;
-  *bytes = plan.bytes;
+  CrossShape shape;
+  if ((rc = plan_cross(di, *st, batch, q_len, kv_len, heads, kv_heads, &shape)) != B200_OK) return rc;
+  *bytes = shape.bytes;
   return B200_OK;
 }
 
@@ -407,8 +466,12 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
   StoredState* st = nullptr;
   if ((rc = current_state(&di, &st)) != B200_OK) return rc;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  CrossShape shape;
+  if ((rc = plan_cross(di, *st, batch, q_len, kv_len, heads, kv_heads, &shape)) != B200_OK ||
+      (rc = check_workspace(workspace, workspace_bytes, shape.bytes)) != B200_OK)
+    return rc;
   CUtensorMap tmK{}, tmV{};
-  if (cross_splits(q_len, heads, kv_heads)) {
+  if (shape.few) {
     b200::SplitAttnParams p{};
     p.batch = (int32_t)batch;
     p.q_len = (int32_t)q_len;
@@ -425,18 +488,20 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
     p.seq_lens = kv_lens;
     p.kv_len = (int32_t)kv_len;
     constexpr uint32_t kBox = b200::SplitPlan<false, 1>::kKeys;
-    SplitPlanHost plan;
-    if ((rc = plan_split_attn(*st, false, batch, p.rows, kv_heads, kv_len, &plan)) != B200_OK) return rc;
     if (kv_len > 0 && ((rc = encode_view(di, &tmK, kk, batch, kv_len, kv_heads, kBox, true)) != B200_OK ||
                        (rc = encode_view(di, &tmV, vv, batch, kv_len, kv_heads, kBox, true)) != B200_OK))
       return rc;
-    return run_split(di, plan, false, tmK, tmV, p, workspace, workspace_bytes, stream);
+    return run_split(di, shape.split, tmK, tmV, p, workspace, stream);
   }
   if (!st->cross_regs_ok) return B200_ERR_CUDA;  // built with another register count: never launch it
   CUtensorMap tmQ, tmO;
-  if ((rc = encode_view(di, &tmQ, qq, batch, q_len, heads, b200::kAttnBQ, true)) != B200_OK ||
-      (rc = encode_view(di, &tmO, oo, batch, q_len, heads, 32, false)) != B200_OK)
-    return rc;
+  if ((rc = encode_view(di, &tmQ, qq, batch, q_len, heads, b200::kAttnBQ, true)) != B200_OK) return rc;
+  const int64_t rows = batch * heads * q_len;
+  float* part_o = static_cast<float*>(workspace);
+  float* part_lse = part_o + (size_t)shape.parts * (size_t)rows * b200::kAttnD;  // (with several parts)
+  rc = shape.parts > 1 ? encode_parts(di, &tmO, part_o, q_len, shape.parts * batch * heads)
+                       : encode_view(di, &tmO, oo, batch, q_len, heads, 32, false);
+  if (rc != B200_OK) return rc;
   if (kv_len > 0) {
     if ((rc = encode_view(di, &tmK, kk, batch, kv_len, kv_heads, b200::kAttnBKV, true)) != B200_OK ||
         (rc = encode_view(di, &tmV, vv, batch, kv_len, kv_heads, 64, true)) != B200_OK)
@@ -455,10 +520,23 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
   p.status = di.status;
   p.kv_len = (int32_t)kv_len;
   p.kv_lens = kv_lens;
-  p.lse = lse;
-  return launch(b200::flash_attn_fwd_kernel<true>,
-                dim3((unsigned)(heads * batch), (unsigned)((p.num_q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles)),
-                b200::kAttnThreads, b200::AttnSmemPlan::kAllocBytes, stream, tmQ, tmK, tmV, tmO, p);
+  p.lse = shape.parts > 1 ? part_lse : lse;
+  const dim3 grid((unsigned)(heads * batch), (unsigned)((p.num_q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles),
+                  (unsigned)shape.parts);
+  rc = launch(b200::flash_attn_fwd_kernel<true>, grid, b200::kAttnThreads, b200::AttnSmemPlan::kAllocBytes, stream, tmQ, tmK,
+              tmV, tmO, p);
+  if (rc != B200_OK || shape.parts == 1) return rc;
+  b200::AttnMergeParams m{};
+  m.part_o = part_o;
+  m.part_lse = part_lse;
+  m.o = static_cast<__nv_bfloat16*>(oo.data);
+  m.o_batch = oo.batch_stride, m.o_seq = oo.seq_stride, m.o_head = oo.head_stride;
+  m.lse = lse;
+  m.parts = shape.parts;
+  m.heads = p.heads;
+  m.q_len = p.seq_len;
+  m.rows = rows;
+  return launch(b200::attn_merge_kernel, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, m);
 }
 
 namespace {
