@@ -48,6 +48,10 @@
 // without keys writes O = 0 and lse = -inf.  A grid that would leave SMs idle is
 // split along the keys (gridDim.z): each part writes its own normalised O in
 // fp32 and its lse, and attn_merge_kernel (attn_split_sm100.cuh) adds the parts.
+// A query tile that is alone in its CTA is worked on by both softmax
+// warpgroups, which take its key tiles in turn (each with S, O, maximum and sum of
+// its own, joined through shared memory at the end): HALVESA us per key tile against 1.6
+// with one of them idle.
 #pragma once
 
 #include <cuda.h>
@@ -328,6 +332,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   }
   const int n_max = max(n0, n1);
+  // One query tile, key tiles t = 0, 2, .. for warpgroup 0 and 1, 3, .. for 1.
+  const bool halves = kCross && n1 == 0 && n0 > 1;
   const int n_q = n1 > 0 ? 2 : (n0 > 0 ? 1 : 0);  // query tiles this CTA reads
 
   if (warp >= kAttnProducerWarp) {
@@ -439,7 +445,46 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         auto wait_k = [&](int j) { return mbar_wait(k_full(k_slot(j)), k_par(j), p.timeout_ns, abort_flag); };
         bool ok = true;
         for (int i = 0; ok && i < n_q; ++i) ok = mbar_wait(q_full(i), 0u, p.timeout_ns, abort_flag);
-        if (ok && n_max > 0) {
+        if constexpr (kCross) {
+          if (halves) {
+            auto issue = [&](int t) {  // S of key tile t, whose only use K has here
+              if (!wait_k(t)) return false;
+              tc_fence_after();
+              const uint32_t kt = sK + (uint32_t)(k_slot(t) * Plan::kTileBytes);
+#pragma unroll
+              for (int k = 0; k < kAttnD / kUmmaK; ++k) {
+                umma_bf16(tmem_base + (uint32_t)((t & 1) * 128), kmajor(sQ, k), kmajor(kt, k), idesc_s, k > 0 ? 1u : 0u);
+              }
+              umma_commit(s_full(t & 1));
+              umma_commit(k_empty(k_slot(t)));
+              return true;
+            };
+            for (int t = 0; t < 2; ++t) ok = ok && issue(t);
+            for (int t = 0; ok && t < n0; ++t) {
+              const int i = t & 1;
+              ok = mbar_wait(v_full(v_slot(t)), v_par(t), p.timeout_ns, abort_flag);
+              for (int h = 0; ok && h < 2; ++h) {
+                ok = mbar_wait(p_full(i, h), (uint32_t)(t >> 1) & 1u, p.timeout_ns, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t vt = sV + (uint32_t)(v_slot(t) * Plan::kTileBytes);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  umma_bf16_ts(tmem_base + 256u + (uint32_t)(i * 128), tmem_base + (uint32_t)(i * 128 + (4 * h + k) * 8),
+                               vdesc(vt, 4 * h + k), idesc_o, (t > 1 || h > 0 || k > 0) ? 1u : 0u);
+                }
+              }
+              if (!ok) break;
+              umma_commit(v_empty(v_slot(t)));
+              if (t + 2 < n0) {
+                ok = issue(t + 2);
+              } else {
+                umma_commit(o_full(i));
+              }
+            }
+          }
+        }
+        if (ok && n_max > 0 && !halves) {
           ok = wait_k(0);
           if (ok) {
             tc_fence_after();
@@ -451,7 +496,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
         const int n_tiles[2] = {n0, n1};
-        for (int j = 0; j < n_max && ok; ++j) {
+        for (int j = 0; j < n_max && ok && !halves; ++j) {
           if (!mbar_wait(v_full(v_slot(j)), v_par(j), p.timeout_ns, abort_flag)) {
             ok = false;
             break;
@@ -525,7 +570,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int qw = warp & 3;                // TMEM lane quarter this warp may access
     const int row = qw * 32 + (int)lane;     // query row in the tile
     const int qt = qt_of[tile];
-    const int n_kv = tile == 0 ? n0 : n1;
+    int n_kv = tile == 0 ? n0 : n1;
+    [[maybe_unused]] int left = kv_len;  // cross attention: keys from this warpgroup's next key tile on
+    if constexpr (kCross) {
+      if (halves) {
+        n_kv = (n0 + 1 - tile) / 2;
+        left = kv_len - tile * kAttnBKV;
+      }
+    }
     const int q_idx = qt * kAttnBQ + row;    // query position
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem_base + lane_off + (uint32_t)(tile * 128);
@@ -557,12 +609,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const bool diag = p.causal && kv0 + kAttnBKV > qt * kAttnBQ;  // the tile crossing the diagonal
       // Only the diagonal tile and a tile past the sequence end need masks:
       // keys c >= lim are masked.
-      const bool masked = diag || kv0 + kAttnBKV > kv_len;
+      const bool masked = kCross ? left < kAttnBKV : diag || kv0 + kAttnBKV > kv_len;
       if (masked) {
-        const int lim = min(kv_len - kv0, diag ? q_idx - kv0 + 1 : kAttnBKV);
+        const int lim = kCross ? left : min(kv_len - kv0, diag ? q_idx - kv0 + 1 : kAttnBKV);
 #pragma unroll
         for (int c = 0; c < kAttnBKV; ++c) x[c] = c < lim ? x[c] : -INFINITY;
       }
+      if constexpr (kCross) left -= halves ? 2 * kAttnBKV : kAttnBKV;
       // Row max of the raw scores (the scale is positive): eight independent
       // chains of three-input maxima, so one thread's row is not one long
       // dependency chain.
@@ -611,8 +664,44 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (lane == 0) mbar_arrive(p_full(tile, h));
       }
     }
+    // Two warpgroups on one query tile: the second hands its O (fp32, over the
+    // K ring, which no product reads any more), maximum and sum (in the second
+    // query tile's buffer, not used) to the first.
+    [[maybe_unused]] const uint32_t other = sK + (uint32_t)row * 512u;
+    [[maybe_unused]] float2* other_ml = reinterpret_cast<float2*>(base_ptr + Plan::kOffQ + Plan::kTileBytes);
+    if constexpr (kCross) {
+      if (halves) {
+        if (tile == 1 && ok) {
+          ok = __all_sync(0xffffffffu, mbar_wait(o_full(1), 0u, p.timeout_ns, abort_flag));
+          if (ok) {
+            tc_fence_after();
+            other_ml[row] = make_float2(m, l);
+#pragma unroll 1
+            for (int c0 = 0; c0 < kAttnD; c0 += 32) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(tO + (uint32_t)c0, r);
+              tmem_ld_wait_regs(r);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {  // 16-byte cells, permuted so that the lanes' stores touch every bank once
+                const uint32_t at = other + (((uint32_t)(c0 / 4 + c) ^ lane) << 4);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[4 * c]), "r"(r[4 * c + 1]),
+                             "r"(r[4 * c + 2]), "r"(r[4 * c + 3])
+                             : "memory");
+              }
+            }
+          }
+        }
+        // Both warpgroups come here whatever happened, and go on only together.
+        const bool both = named_bar_and(2, 256, ok);
+        if (ok && !both && lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
+        if (tile == 1) n_kv = -1;  // nothing more to do
+        ok = ok && both;
+      }
+    }
     if (!ok) {
       if (lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
+    } else if (kCross && n_kv < 0) {
+      // (the second warpgroup of a shared query tile)
     } else if (n_kv > 0) {
       // O / l -> bf16 -> TMA store, through this warp's 8 KiB of the tile's
       // Q buffer (idle once the last product is done): two [32 rows][64 d]
@@ -620,6 +709,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const bool last = mbar_wait(o_full(tile), 0u, p.timeout_ns, abort_flag);
       if (__all_sync(0xffffffffu, last)) {
         tc_fence_after();
+        [[maybe_unused]] float mine = 1.0f, theirs = 0.0f;  // factors of the two warpgroups' O
+        if constexpr (kCross) {
+          if (halves) {
+            const float2 ml = other_ml[row];
+            const float top = fmaxf(m, ml.x);
+            mine = fast_exp2(m - top);
+            theirs = fast_exp2(ml.x - top);
+            l = l * mine + ml.y * theirs;
+            m = top;
+          }
+        }
         const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
         if constexpr (kCross) {
           if (p.lse != nullptr && q_idx < p.seq_len) {
@@ -635,6 +735,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           tmem_ld_32x32b_x32(tO + (uint32_t)(half * 64 + 32), hi);
           tmem_ld_wait_regs(lo);
           tmem_ld_wait_regs(hi);
+          if constexpr (kCross) {
+            if (halves) {
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                float v[4];
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                             : "r"(other + (((uint32_t)(16 * half + c) ^ lane) << 4))
+                             : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  uint32_t& o = c < 8 ? lo[4 * c + i] : hi[4 * (c - 8) + i];
+                  o = __float_as_uint(__uint_as_float(o) * mine + v[i] * theirs);
+                }
+              }
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             lo[i] = __float_as_uint(__uint_as_float(lo[i]) * inv_l);

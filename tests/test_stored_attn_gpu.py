@@ -453,10 +453,13 @@ def test_cross_attn_growing_scores():
         _cross_check(q, k, v)
 
 
-def test_cross_attn_equals_flash_attn_on_square_shapes():
-    g = torch.Generator().manual_seed(21)
-    q, k, v = (_randn(g, 2, 384, h, 128).to(DEV) for h in (4, 2, 2))
-    assert torch.equal(b200_gemm.cross_attn(q, k, v), b200_gemm.flash_attn(q, k, v, causal=False))
+def test_cross_attn_agrees_with_flash_attn_on_square_shapes():
+    """The same function: both within the bound of the exact result (their key tiles may be added in another order)."""
+    for n in (384, 512):
+        q, k, v = _cross_inputs(21 + n, 2, n, n, 4, 2)
+        want = ref.cross_attn(q, k, v)["out"]
+        _within(b200_gemm.cross_attn(*_on([q, k, v])), *want, "cross")
+        _within(b200_gemm.flash_attn(*_on([q, k, v]), causal=False), *want, "flash")
     _ok()
 
 
