@@ -64,6 +64,7 @@ struct AttnBwdParams {
   int32_t q_len, kv_len, heads, kv_heads, group, batch;
   int32_t q_tiles, kv_tiles;
   int32_t items;           // of this kernel's kind
+  uint32_t ordered;        // entries by falling number of keys (more items than SMs, at most 32 entries)
   uint32_t early;          // dQ: launched behind the dK/dV kernel, of which it needs nothing
   const int32_t* kv_lens;  // [batch] or NULL
   float scale, scale_log2;
@@ -149,7 +150,8 @@ struct AttnBwdPlan {
   static constexpr int kOffBar = kOffOut + (kDQ ? 0 : 8 * 2048);
   static constexpr int kNumBars = 2 + 3 * kY1Stages + 2 * kY2Stages + 2 + 1 + 1 + 1 + 2 + 1 + 1 + 4;
   static constexpr int kOffItem = kOffBar + kNumBars * 8;  // two slots of (item or -1, keys of its entry)
-  static constexpr int kOffTmemHolder = kOffItem + 16;
+  static constexpr int kOffOrder = kOffItem + 16;  // batches of up to 32: the entries by falling number of keys
+  static constexpr int kOffTmemHolder = kOffOrder + 32 * 4;
   static constexpr int kOffAbort = kOffTmemHolder + 4;
   static constexpr int kBytes = kOffAbort + 4;
   static constexpr int kAllocBytes = kBytes + 1024;
@@ -275,6 +277,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto item_full = [&](uint32_t k) { return bar0 + 8u * (kB + 9 + (k & 1u)); };
   auto item_empty = [&](uint32_t k) { return bar0 + 8u * (kB + 11 + (k & 1u)); };
   volatile int2* items = reinterpret_cast<volatile int2*>(base_ptr + Plan::kOffItem);
+  volatile int32_t* order = reinterpret_cast<volatile int32_t*>(base_ptr + Plan::kOffOrder);
   volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffTmemHolder);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffAbort);
 
@@ -324,9 +327,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   // needs no wait of its own (until the end, below).
   if (!(kDQ && p.early != 0u)) pdl_wait();
   pdl_launch_dependents();
+  if (p.ordered) {
+    if (warp < 8) {
+      for (int slot = warp; slot < p.batch; slot += 8) {
+        const int e = attn_entry_by_length(p.kv_lens, p.batch, p.kv_len, slot);
+        if (lane == 0) order[slot] = e;
+      }
+    }
+    __syncthreads();
+  }
 
   // An item: its tile, head and entry, and the number of tiles to stream.
-  // Tiles change fastest: neighbours stream the same tiles.  (Entries fastest, so
+  // Entries with many keys come first, so that the last items are short.  Tiles
+  // change fastest: neighbours stream the same tiles.  (Entries fastest, so
   // that long and short ones alternate: 4 % slower on 8 ragged pairs.)
   struct Item {
     int tile, head, bat, kv_len, n;
@@ -338,6 +351,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     t.tile = id % tiles;
     t.head = (id / tiles) % heads;
     t.bat = (id / tiles) / heads;
+    if (p.ordered) t.bat = order[t.bat];
     t.kv_len = kv_len;
     const int kv_tiles = (kv_len + 127) / 128;
     t.n = kDQ ? kv_tiles : (t.tile < kv_tiles ? p.group * p.q_tiles : 0);
@@ -383,7 +397,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             break;
           }
           const bool end = id >= p.items;
-          const int bat = end ? 0 : id / (kDQ ? p.q_tiles * p.heads : p.kv_tiles * p.kv_heads);
+          int bat = end ? 0 : id / (kDQ ? p.q_tiles * p.heads : p.kv_tiles * p.kv_heads);
+          if (p.ordered) bat = order[bat];
           const int kv_len = end ? 0 : attn_kv_len(p.kv_lens, bat, p.kv_len);
           items[k & 1u].x = end ? -1 : id;
           items[k & 1u].y = kv_len;

@@ -258,32 +258,33 @@ int plan_cross(const b200::DeviceInfo& di, const StoredState& st, int64_t batch,
   const int64_t q_tiles = (q_len + b200::kAttnBQ - 1) / b200::kAttnBQ;
   const int64_t ctas = heads * batch * ((q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles);
   const int64_t tiles = (kv_len + b200::kAttnBKV - 1) / b200::kAttnBKV;
-  // On a B200 a query tile takes 1.6 us per key tile alone and two together 1.95,
-  // besides 5.5 us to start and end.  While parts fit beside each other (of two
+  // On a B200 a query tile takes 1.1 us per key tile alone and two together 1.95,
+  // besides 6 us to start and end.  While parts fit beside each other (of two
   // key tiles at least) they save tiles, but cost 4 us for the merge and their
   // O once out and once back, 1 KiB a row and part at 4 TB/s.  Measured: 128 queries, 4
   // heads, 4000 keys: 16 parts 13 us against one 56; 256 queries, 2 x 32 heads,
   // 1000 keys: 2 parts 26 against 21.
   const int64_t rows = batch * heads * q_len;
-  const double per_tile = q_tiles == 1 ? 1.6 : 1.95;
+  const double per_tile = q_tiles == 1 ? 1.1 : 1.95;
   const double waves = std::ceil((double)ctas / di.sm_count);
-  double tc = 5.5 + waves * (double)tiles * per_tile;
+  double tc = 6.0 + waves * (double)tiles * per_tile;
   const int64_t most = ctas < di.sm_count ? std::min(di.sm_count / ctas, tiles / 2) : 1;
   for (int64_t n = 2; n <= most; ++n) {
-    const double t = 9.5 + (double)((tiles + n - 1) / n) * per_tile + 1024.0 * (double)(rows * n) / 4e6;
+    const double t = 10.0 + (double)((tiles + n - 1) / n) * per_tile + 1024.0 * (double)(rows * n) / 4e6;
     if (t < tc) {
       tc = t;
       out->parts = (int)n;
     }
   }
-  // The split kernel reads K and V once, at 5.6 TB/s, besides 9.5 us.  It takes up
-  // to 16 rows per key/value head (with two row tiles per warp it lost to the
-  // tcgen05 kernel in parts: 32 rows, 4 heads, 1000 keys 17 against 11 us).  Measured:
-  // one query, 4 heads: 9.9 against 7.0 us (tcgen05) at 200 keys, 10.4 against 16.8 at
-  // 1000 (one part); 8 x 16 heads, 4000 keys: 52 against 58.
+  // The split kernel reads K and V once, at 5.6 TB/s, besides 9.5 us (the tcgen05
+  // kernel at 4.8 at most, one CTA per SM).  It takes up to 16 rows per key/value
+  // head (with two row tiles per warp it lost to the tcgen05 kernel in parts:
+  // 32 rows, 4 heads, 1000 keys 17 against 11 us).  Measured: one query, 4 heads: 9.9
+  // against 7.0 us (tcgen05) at 200 keys, 10.4 against 16.8 at 1000 (one part); 32 x 16
+  // heads, 200 to 2000 keys: 57 against 69.
   if (q_len * (heads / kv_heads) <= 16) {
-    const double split = 9.5 + 4.0 * b200::kKvD * (double)batch * (double)kv_heads * (double)kv_len / 5.6e6;
-    out->few = split < tc;
+    const double bytes = 4.0 * b200::kKvD * (double)batch * (double)kv_heads * (double)kv_len;
+    out->few = 9.5 + bytes / 5.6e6 < std::max(tc, 6.0 + bytes / 4.8e6);
   }
   if (out->few) {
     out->parts = 1;
@@ -520,6 +521,10 @@ extern "C" B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200
   p.status = di.status;
   p.kv_len = (int32_t)kv_len;
   p.kv_lens = kv_lens;
+  p.ordered = kv_lens != nullptr && batch > 1 && batch <= 32 &&
+                      heads * batch * ((p.num_q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles) > di.sm_count
+                  ? 1u
+                  : 0u;
   p.lse = shape.parts > 1 ? part_lse : lse;
   const dim3 grid((unsigned)(heads * batch), (unsigned)((p.num_q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles),
                   (unsigned)shape.parts);
@@ -642,8 +647,12 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   const dim3 grid((unsigned)std::max<int64_t>(q_tiles * 2, 1), (unsigned)std::min<int64_t>(rows, 65535),
                   (unsigned)((rows + 65534) / 65535));
   if ((rc = launch(b200::attn_bwd_delta_kernel, grid, 256, 0, stream, d)) != B200_OK) return rc;
+  auto order = [&](int64_t items) {
+    return kv_lens != nullptr && batch > 1 && batch <= 32 && items > di.sm_count ? 1u : 0u;
+  };
   if (dkv_items > 0) {
     p.items = (int32_t)dkv_items;
+    p.ordered = order(dkv_items);
     p.counter = counters;
     if ((rc = launch(b200::attn_bwd_kernel<false>, dim3((unsigned)std::min<int64_t>(dkv_items, di.sm_count)),
                      b200::kAttnThreads, b200::AttnBwdPlan<false>::kAllocBytes, stream, tm, p)) != B200_OK)
@@ -651,6 +660,7 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   }
   if (dq_items > 0) {
     p.items = (int32_t)dq_items;
+    p.ordered = order(dq_items);
     p.counter = counters + 1;
     p.early = dkv_items > 0 ? 1u : 0u;
     rc = launch(b200::attn_bwd_kernel<true>, dim3((unsigned)std::min<int64_t>(dq_items, di.sm_count)), b200::kAttnThreads,
