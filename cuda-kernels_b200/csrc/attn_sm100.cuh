@@ -360,8 +360,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
   const int n_max = max(n0, n1);
   // One query tile, key tiles t = 0, 2, .. for warpgroup 0 and 1, 3, .. for 1.
-  // (From three on: the join takes 0.6 us.)
-  const bool halves = kCross && n1 == 0 && n0 > 2;
+  const bool halves = kCross && n1 == 0 && n0 > 1;
   const int n_q = n1 > 0 ? 2 : (n0 > 0 ? 1 : 0);  // query tiles this CTA reads
 
   if (warp >= kAttnProducerWarp) {
@@ -597,11 +596,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int tile = warp >> 2;
     const int qw = warp & 3;                // TMEM lane quarter this warp may access
     const int row = qw * 32 + (int)lane;     // query row in the tile
-    const int qt = qt_of[tile];
+    int qt = qt_of[tile];
     int n_kv = tile == 0 ? n0 : n1;
     [[maybe_unused]] int left = kv_len;  // cross attention: keys from this warpgroup's next key tile on
     if constexpr (kCross) {
       if (halves) {
+        qt = qt_of[0];
         n_kv = (n0 + 1 - tile) / 2;
         left = kv_len - tile * kAttnBKV;
       }
@@ -692,44 +692,29 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (lane == 0) mbar_arrive(p_full(tile, h));
       }
     }
-    // Two warpgroups on one query tile: the second hands its O (fp32, over the
-    // K ring, which no product reads any more), maximum and sum (in the second
-    // query tile's buffer, not used) to the first.
-    [[maybe_unused]] const uint32_t other = sK + (uint32_t)row * 512u;
-    [[maybe_unused]] float2* other_ml = reinterpret_cast<float2*>(base_ptr + Plan::kOffQ + Plan::kTileBytes);
+    // Two warpgroups on one query tile: they tell each other maximum and sum
+    // (through the second query tile's buffer, not used), and each joins 64
+    // columns of the two O, which lie in the same lanes of TMEM.
+    [[maybe_unused]] float mine = 1.0f, theirs = 0.0f;  // factors of this and the other warpgroup's O
     if constexpr (kCross) {
       if (halves) {
-        if (tile == 1 && ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait(o_full(1), 0u, p.timeout_ns, abort_flag));
-          if (ok) {
-            tc_fence_after();
-            other_ml[row] = make_float2(m, l);
-#pragma unroll 1
-            for (int c0 = 0; c0 < kAttnD; c0 += 32) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(tO + (uint32_t)c0, r);
-              tmem_ld_wait_regs(r);
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {  // 16-byte cells, permuted so that the lanes' stores touch every bank once
-                const uint32_t at = other + (((uint32_t)(c0 / 4 + c) ^ lane) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[4 * c]), "r"(r[4 * c + 1]),
-                             "r"(r[4 * c + 2]), "r"(r[4 * c + 3])
-                             : "memory");
-              }
-            }
-          }
-        }
+        float2* ml = reinterpret_cast<float2*>(base_ptr + Plan::kOffQ + Plan::kTileBytes);
+        ml[tile * 128 + row] = make_float2(m, l);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full(1 - tile), 0u, p.timeout_ns, abort_flag));
         // Both warpgroups come here whatever happened, and go on only together.
         const bool both = named_bar_and(2, 256, ok);
-        if (ok && !both && lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
-        if (tile == 1) n_kv = -1;  // nothing more to do
-        ok = ok && both;
+        const float2 other = ml[(1 - tile) * 128 + row];
+        const float top = fmaxf(m, other.x);
+        mine = fast_exp2(m - top);
+        theirs = fast_exp2(other.x - top);
+        l = l * mine + other.y * theirs;
+        m = top;
+        ok = both;
+        named_bar_sync(2, 256);  // both have read, before a buffer is staged over
       }
     }
     if (!ok) {
       if (lane == 0) attn_raise(p, abort_flag, kDevTimeoutEpilogue);
-    } else if (kCross && n_kv < 0) {
-      // (the second warpgroup of a shared query tile)
     } else if (n_kv > 0) {
       // O / l -> bf16 -> TMA store, through this warp's 8 KiB of the tile's
       // Q buffer (idle once the last product is done): two [32 rows][64 d]
@@ -737,27 +722,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const bool last = mbar_wait(o_full(tile), 0u, p.timeout_ns, abort_flag);
       if (__all_sync(0xffffffffu, last)) {
         tc_fence_after();
-        [[maybe_unused]] float mine = 1.0f, theirs = 0.0f;  // factors of the two warpgroups' O
-        if constexpr (kCross) {
-          if (halves) {
-            const float2 ml = other_ml[row];
-            const float top = fmaxf(m, ml.x);
-            mine = fast_exp2(m - top);
-            theirs = fast_exp2(ml.x - top);
-            l = l * mine + ml.y * theirs;
-            m = top;
-          }
-        }
         const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
         if constexpr (kCross) {
-          if (p.lse != nullptr && q_idx < p.seq_len) {
+          if (p.lse != nullptr && q_idx < p.seq_len && !(halves && tile == 1)) {
             p.lse[(((size_t)blockIdx.z * p.batch + bat) * p.heads + head) * p.seq_len + q_idx] =
                 l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
         }
         const uint32_t stage = sQ + (uint32_t)(tile * Plan::kTileBytes + qw * 8192);
+        const int half0 = halves ? tile : 0, half1 = halves ? tile + 1 : 2;  // 64 columns each
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
+        for (int half = half0; half < half1; ++half) {
           uint32_t lo[32], hi[32];
           tmem_ld_32x32b_x32(tO + (uint32_t)(half * 64), lo);
           tmem_ld_32x32b_x32(tO + (uint32_t)(half * 64 + 32), hi);
@@ -765,18 +740,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           tmem_ld_wait_regs(hi);
           if constexpr (kCross) {
             if (halves) {
+              uint32_t r[32];
+              const uint32_t tX = tmem_base + lane_off + 256u + (uint32_t)((1 - tile) * 128 + half * 64);
+              tmem_ld_32x32b_x32(tX, r);
+              tmem_ld_wait_regs(r);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                float v[4];
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                             : "r"(other + (((uint32_t)(16 * half + c) ^ lane) << 4))
-                             : "memory");
+              for (int i = 0; i < 32; ++i) {
+                lo[i] = __float_as_uint(__uint_as_float(lo[i]) * mine + __uint_as_float(r[i]) * theirs);
+              }
+              tmem_ld_32x32b_x32(tX + 32u, r);
+              tmem_ld_wait_regs(r);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  uint32_t& o = c < 8 ? lo[4 * c + i] : hi[4 * (c - 8) + i];
-                  o = __float_as_uint(__uint_as_float(o) * mine + v[i] * theirs);
-                }
+              for (int i = 0; i < 32; ++i) {
+                hi[i] = __float_as_uint(__uint_as_float(hi[i]) * mine + __uint_as_float(r[i]) * theirs);
               }
             }
           }
@@ -807,7 +783,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0 && !(kCross && gridDim.z > 1)) {
-          for (int half = 0; half < 2; ++half) {
+          for (int half = half0; half < half1; ++half) {
             if constexpr (kCross) {
               tma_store_4d(&tmO, stage + (uint32_t)(half * 4096), 64 * half, head, qt * kAttnBQ + qw * 32, bat);
             } else {
