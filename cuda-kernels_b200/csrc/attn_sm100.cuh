@@ -276,19 +276,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   int bat = (int)blockIdx.x / p.heads;
   int cta_row = (int)blockIdx.y;
   if constexpr (kCross) {
-    // Blocks in the order of their entry's slot, then CTA row, then head: with
-    // lengths on the device the slots are given to entries below.
+    // The longest first: CTAs of two query tiles by their entry's slot (with
+    // lengths on the device the slots are given to entries below), then those of one.
     const int64_t id = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-    head = (int)(id % p.heads);
-    cta_row = (int)(id / p.heads % gridDim.y);
-    bat = (int)(id / p.heads / gridDim.y);
+    const int rows = p.num_q_tiles / kAttnQTiles;
+    const int64_t full = (int64_t)rows * gridDim.x;
+    head = (int)(id % p.heads);  // (gridDim.x is a multiple of the heads)
+    const int64_t rest = (id < full ? id : id - full) / p.heads;
+    cta_row = id < full ? (int)(rest % rows) : rows;
+    bat = (int)(id < full ? rest / rows : rest);
   }
   if (p.balanced) {
     qt_of[0] = (int)blockIdx.y;
     qt_of[1] = p.num_q_tiles - 1 - (int)blockIdx.y;
     if (qt_of[1] <= qt_of[0]) qt_of[1] = p.num_q_tiles;  // the middle tile of an odd count stays alone
   } else {
-    // (Without a causal mask the last CTA row is the shorter one, if any.)
     qt_of[0] = kAttnQTiles * (kCross ? cta_row : (int)gridDim.y - 1 - cta_row);
     qt_of[1] = qt_of[0] + 1;
   }
