@@ -24,7 +24,8 @@ constexpr size_t kWsAlign = 256;
 
 using SplitKernel = void (*)(const CUtensorMap, const CUtensorMap, const b200::SplitAttnParams);
 struct SplitVariant {
-  SplitKernel kernel;
+  SplitKernel kernel;   // the line of units over all warps
+  SplitKernel cluster;  // a cluster per segment
   void (*join)(const b200::SplitAttnParams);
   int tiles;  // row tiles per warp
   int smem;
@@ -33,16 +34,17 @@ struct SplitVariant {
 // bf16 states of few query rows; the 8-bit cache with one or two row tiles per warp.
 enum SplitIndex { kSplitBf16 = 0, kSplitFp8 = 1, kSplitFp8Wide = 2, kSplitVariants = 3 };
 const SplitVariant kSplit[kSplitVariants] = {
-    {b200::attn_split_kernel<false, 1>, b200::attn_join_kernel<1>, 1, b200::SplitPlan<false, 1>::kAllocBytes,
+    {b200::attn_split_kernel<false, 1, false>, b200::attn_split_kernel<false, 1, true>, b200::attn_join_kernel<1>, 1, b200::SplitPlan<false, 1>::kAllocBytes,
      b200::SplitPlan<false, 1>::kPartFloats},
-    {b200::attn_split_kernel<true, 1>, b200::attn_join_kernel<1>, 1, b200::SplitPlan<true, 1>::kAllocBytes,
+    {b200::attn_split_kernel<true, 1, false>, b200::attn_split_kernel<true, 1, true>, b200::attn_join_kernel<1>, 1, b200::SplitPlan<true, 1>::kAllocBytes,
      b200::SplitPlan<true, 1>::kPartFloats},
-    {b200::attn_split_kernel<true, 2>, b200::attn_join_kernel<2>, 2, b200::SplitPlan<true, 2>::kAllocBytes,
+    {b200::attn_split_kernel<true, 2, false>, b200::attn_split_kernel<true, 2, true>, b200::attn_join_kernel<2>, 2, b200::SplitPlan<true, 2>::kAllocBytes,
      b200::SplitPlan<true, 2>::kPartFloats}};
 
 struct StoredState {
   std::once_flag once;
   int init_rc = B200_OK;
+  int sm_count = 0;
   bool cross_regs_ok = false, bwd_regs_ok = false;  // setmaxnreg shares match the binary (attn_sm100.cuh)
   int split_ctas[kSplitVariants] = {};  // resident CTAs of each split variant on the whole GPU
 };
@@ -54,6 +56,7 @@ int init_stored(const b200::DeviceInfo& di, StoredState& st) {
     return B200_ERR_CUDA;
   cudaFuncAttributes fa{};
   if (cudaFuncGetAttributes(&fa, b200::flash_attn_fwd_kernel<true>) != cudaSuccess) return B200_ERR_CUDA;
+  st.sm_count = di.sm_count;
   st.cross_regs_ok = fa.numRegs == (int)b200::kAttnRegsLaunch;
   st.bwd_regs_ok = true;
   const std::pair<const void*, int> bwd[2] = {
@@ -69,6 +72,7 @@ int init_stored(const b200::DeviceInfo& di, StoredState& st) {
     const SplitVariant& v = kSplit[i];
     int per_sm = 0;
     if (cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess ||
+        cudaFuncSetAttribute(v.cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.kernel, b200::kSplitThreads, v.smem) != cudaSuccess ||
         per_sm < 1)
       return B200_ERR_CUDA;
@@ -147,20 +151,29 @@ int encode_parts(const b200::DeviceInfo& di, CUtensorMap* map, float* data, int6
 }
 
 template <typename... Params, typename... Args>
-int launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+int launch_clusters(void (*kernel)(Params...), int cluster, dim3 grid, int threads, int smem, cudaStream_t stream,
+                    const Args&... args) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return B200_OK;
   cudaGetLastError();
   return B200_ERR_CUDA;
+}
+template <typename... Params, typename... Args>
+int launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+  return launch_clusters(kernel, 1, grid, threads, smem, stream, args...);
 }
 
 int check_heads(int64_t batch, int64_t q_len, int64_t heads, int64_t kv_heads, int64_t head_dim) {
@@ -195,6 +208,8 @@ int check_cache_pointers(const b200_kv_cache* c) {
 struct SplitShape {
   SplitIndex index;
   int64_t row_tiles;
+  int cluster;  // CTAs per segment, 0: the line
+  int each;     // units per warp of a cluster
   int ctas;
   bool cut;  // some segment can be longer than a unit: partial results need the workspace
   size_t bytes;
@@ -208,8 +223,26 @@ int plan_split(const StoredState& st, SplitIndex index, int64_t batch, int64_t r
   const int64_t units = (kv_len + keys - 1) / keys;          // of the longest segment
   const int64_t segs = kv_heads * out->row_tiles;
   if (segs > kLim) return B200_ERR_TOO_LARGE;
-  // One worker per unit at most (in double: the product may pass 2^63).
-  const double most = (double)batch * (double)segs * (double)std::max<int64_t>(units, 1);
+  const double all_segs = (double)batch * (double)segs;  // (in double: the products may pass 2^63)
+  // A cluster per segment, large enough for a unit per warp if the clusters
+  // still fit two CTAs to an SM, while its warps have few units.  Measured on a B200, 8-bit
+  // cache: 8 segments of 1000 keys 7.8 us against 12.9 along the line, of 4000 11.8
+  // against 14.9; 128 of 1000 16.2 against 22.1, of 2000 24.7 against 27.5, of 4000 41.9
+  // against 37.5; 512 of 250 18.0 against 21.9, of 1000 37.7 against 38.5, of 2000 62 against 59.
+  int cluster = 1;
+  while (cluster < 8 && b200::kSplitWarps * cluster < units && 2 * cluster * all_segs <= 2.0 * st.sm_count) cluster *= 2;
+  const int64_t each = (units + b200::kSplitWarps * cluster - 1) / (b200::kSplitWarps * cluster);  // units per warp
+  out->cluster = 0;
+  if (each <= (cluster == 8 ? 4 : 8) && all_segs * cluster <= (double)kLim) {
+    out->cluster = cluster;
+    out->each = (int)each;
+    out->ctas = (int)(all_segs * cluster);
+    out->cut = false;
+    out->bytes = 0;
+    return B200_OK;
+  }
+  // One worker per unit at most.
+  const double most = all_segs * (double)std::max<int64_t>(units, 1);
   out->ctas = (int)std::min((double)st.split_ctas[index], std::ceil(most / b200::kSplitWarps));
   out->cut = units > 1;
   out->bytes = out->cut ? (size_t)(out->ctas * b200::kSplitWarps) * (2 * v.part_floats * sizeof(float) + sizeof(int4)) : 0;
@@ -235,6 +268,10 @@ int run_split(const b200::DeviceInfo& di, const SplitShape& shape, const CUtenso
   p.workers = workers;
   p.timeout_ns = di.timeout_ns;
   p.status = di.status;
+  if (shape.cluster > 0) {
+    return launch_clusters(v.cluster, shape.cluster, dim3((unsigned)shape.ctas), b200::kSplitThreads, v.smem, stream, tmK,
+                           tmV, p);
+  }
   const int rc = launch(v.kernel, dim3((unsigned)shape.ctas), b200::kSplitThreads, v.smem, stream, tmK, tmV, p);
   if (rc != B200_OK || !shape.cut) return rc;
   const int rows = std::min<int>(p.rows, 16 * v.tiles);
@@ -258,39 +295,48 @@ int plan_cross(const b200::DeviceInfo& di, const StoredState& st, int64_t batch,
   const int64_t q_tiles = (q_len + b200::kAttnBQ - 1) / b200::kAttnBQ;
   const int64_t ctas = heads * batch * ((q_tiles + b200::kAttnQTiles - 1) / b200::kAttnQTiles);
   const int64_t tiles = (kv_len + b200::kAttnBKV - 1) / b200::kAttnBKV;
-  // On a B200 a query tile takes 1.1 us per key tile alone and two together 1.95,
-  // besides 6 us to start and end.  While parts fit beside each other (of two
-  // key tiles at least) they save tiles, but cost 4 us for the merge and their
-  // O once out and once back, 1 KiB a row and part at 4 TB/s.  Measured: 128 queries, 4
-  // heads, 4000 keys: 16 parts 13 us against one 56; 256 queries, 2 x 32 heads,
-  // 1000 keys: 2 parts 26 against 21.
+  // The tcgen05 kernel, on a B200: 5 us a wave of CTAs to start and end, and per key
+  // tile 1.1 us for a query tile alone and 1.95 for two together; K and V at 5.6
+  // TB/s at most, 4.8 in several waves.  While parts fit beside each other (of two
+  // key tiles at least) they save tiles, but cost 3.8 us for the merge and their O once out and once
+  // back, 1 KiB a row and part at 4 TB/s.  Measured: 128 queries, 4 heads, 4000
+  // keys: 16 parts 13 us against one 56; 256 queries, 2 x 32 heads, 1000 keys: 2 parts 26
+  // against 21.
   const int64_t rows = batch * heads * q_len;
+  const double bytes = 4.0 * b200::kKvD * (double)batch * (double)kv_heads * (double)kv_len;  // of K and V
   const double per_tile = q_tiles == 1 ? 1.1 : 1.95;
   const double waves = std::ceil((double)ctas / di.sm_count);
-  double tc = 6.0 + waves * (double)tiles * per_tile;
+  double tc = waves * (5.0 + (double)tiles * per_tile);
   const int64_t most = ctas < di.sm_count ? std::min(di.sm_count / ctas, tiles / 2) : 1;
   for (int64_t n = 2; n <= most; ++n) {
-    const double t = 10.0 + (double)((tiles + n - 1) / n) * per_tile + 1024.0 * (double)(rows * n) / 4e6;
+    const double t = 8.8 + (double)((tiles + n - 1) / n) * per_tile + 1024.0 * (double)(rows * n) / 4e6;
     if (t < tc) {
       tc = t;
       out->parts = (int)n;
     }
   }
-  // The split kernel reads K and V once, at 5.6 TB/s, besides 9.5 us (the tcgen05
-  // kernel at 4.8 at most, one CTA per SM).  It takes up to 16 rows per key/value
-  // head (with two row tiles per warp it lost to the tcgen05 kernel in parts:
-  // 32 rows, 4 heads, 1000 keys 17 against 11 us).  Measured: one query, 4 heads: 9.9
-  // against 7.0 us (tcgen05) at 200 keys, 10.4 against 16.8 at 1000 (one part); 32 x 16
-  // heads, 200 to 2000 keys: 57 against 69.
-  if (q_len * (heads / kv_heads) <= 16) {
-    const double bytes = 4.0 * b200::kKvD * (double)batch * (double)kv_heads * (double)kv_len;
-    out->few = 9.5 + bytes / 5.6e6 < std::max(tc, 6.0 + bytes / 4.8e6);
+  tc = std::max(tc, 3.0 + bytes / (waves > 1.0 ? 4.8e6 : 5.6e6));
+  // The split kernel, for up to 16 rows per key/value head (two row tiles per
+  // warp lost to the tcgen05 kernel in parts: 32 rows, 4 heads, 1000 keys 17 us
+  // against 11): in clusters 3.5 us, 0.6 for each doubling, 1.25 per unit of a warp,
+  // and K and V, partly beside that; along the line 9.5 us and K and V at 5.6 TB/s; with
+  // more than 8 rows 1.2 to 4.2 us more for their queries and outputs.  Measured, split against tcgen05: one query, 16 heads, 128 keys
+  // 4.4 us against 5.4, 1000 keys 6.8 against 10.1; 8 x 16 heads, 4000 keys 54 against
+  // 47; 16 queries, 8 x 16 heads, 128 keys 9.5 against 6.2.
+  const int64_t group_rows = q_len * (heads / kv_heads);
+  if (group_rows <= 16) {
+    const int rc = plan_split(st, kSplitBf16, batch, group_rows, kv_heads, kv_len, &out->split);
+    if (rc != B200_OK) return rc;
+    const double split = (out->split.cluster > 0 ? 3.5 + 0.6 * std::log2((double)out->split.cluster) +
+                                                       1.25 * out->split.each + bytes / 1.2e7
+                                                 : 9.5 + bytes / 5.6e6) +
+                         (group_rows > 8 ? 1.2 + std::min(3.0, 0.07 * (double)(batch * kv_heads)) : 0.0);
+    out->few = split < tc;
   }
   if (out->few) {
     out->parts = 1;
-    const int rc = plan_split(st, kSplitBf16, batch, q_len * (heads / kv_heads), kv_heads, kv_len, &out->split);
     out->bytes = out->split.bytes;
-    return rc;
+    return B200_OK;
   }
   if (out->parts > 1) out->bytes = (size_t)out->parts * (size_t)(batch * heads * q_len) * (b200::kAttnD + 1) * sizeof(float);
   out->bytes = (out->bytes + kWsAlign - 1) / kWsAlign * kWsAlign;
