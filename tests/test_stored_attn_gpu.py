@@ -285,6 +285,51 @@ def test_cache_attn_large_batch():
     _within(out, want, bound)
 
 
+@pytest.mark.parametrize("shape", [(1, 4, 4), (1, 32, 1), (5, 16, 2), (9, 8, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_cache_attn_short_sequences_under_a_wide_table(shape):
+    """The table has room for 64 times the tokens there are; entries of no page hold -1 and are not read."""
+    t, h, kv = shape
+    g = torch.Generator().manual_seed(70 + h)
+    lens = [0, 1, 31, 32, 33, 64, 0, 300, 1000, 0]
+    cache = _filled(g, lens, kv, 32)
+    wide = torch.full((len(lens), 2000), -1, dtype=torch.int32)
+    for i, n in enumerate(lens):
+        wide[i, :-(-n // 32)] = cache[4][i, :-(-n // 32)]
+    cache[4] = wide
+    q = _randn(g, len(lens), t, h, 128)
+    out = b200_gemm.cache_attn(q.to(DEV), *_on(cache))
+    _ok()
+    want, bound = ref.cache_attn(q, *cache)
+    _within(out, want, bound)
+
+
+@pytest.mark.parametrize("shape", [(1, 8, 2), (6, 8, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_cache_attn_long_and_short_side_by_side(shape):
+    """Workers that hold the end of a long sequence, several short ones and the start of the next; up to 48 rows."""
+    t, h, kv = shape
+    g = torch.Generator().manual_seed(80 + h)
+    lens = [9000, 0, 3, 40, 12345, 1, 0, 700, 16000]
+    cache = _filled(g, lens, kv, 128)
+    q = _randn(g, len(lens), t, h, 128)
+    out = b200_gemm.cache_attn(q.to(DEV), *_on(cache))
+    _ok()
+    want, bound = ref.cache_attn(q, *cache)
+    _within(out, want, bound)
+
+
+def test_cache_attn_sequences_that_share_pages():
+    """A common prefix stored once: the same pages in several rows of the table."""
+    g = torch.Generator().manual_seed(90)
+    cache = _filled(g, [200, 180, 64], 2, 32)
+    cache[4][1, :2] = cache[4][0, :2]
+    cache[4][2, :2] = cache[4][0, :2]
+    q = _randn(g, 3, 1, 8, 128)
+    out = b200_gemm.cache_attn(q.to(DEV), *_on(cache))
+    _ok()
+    want, bound = ref.cache_attn(q, *cache)
+    _within(out, want, bound)
+
+
 def test_cache_attn_offsets_past_32_bits():
     """A cache of 4.5 GB each for K and V, the sequence's pages at its far end."""
     g = torch.Generator().manual_seed(17)
@@ -413,6 +458,24 @@ def test_cross_attn_ragged_sources(t):
     _cross_check(q, _spoil(k, lens), _spoil(v, lens), lens)
 
 
+@pytest.mark.parametrize("t", [1, 4, 100, 200])
+@pytest.mark.parametrize("lens", [[0, 1, 31, 32, 33, 4000, 8999, 9000], [0, 0, 1, 0, 5, 130, 0, 0]], ids=["mixed", "short"])
+def test_cross_attn_ragged_long_sources(t, lens):
+    """Few rows per key/value head: workers or parts along the keys, most of which have no keys of a short source."""
+    q, k, v = _cross_inputs(t + len(lens), len(lens), t, 9000, 8 if t < 100 else 2, 2 if t < 100 else 1)
+    _cross_check(q, _spoil(k, lens), _spoil(v, lens), lens)
+
+
+@pytest.mark.parametrize("batch,heads", [(12, (16, 4)), (40, (8, 8))], ids=["few entries", "many entries"])
+@pytest.mark.parametrize("t", [100, 300])
+def test_cross_attn_more_work_than_sms(t, batch, heads):
+    """Several CTAs per SM, entries of many and of no keys among them."""
+    lens = [(i * 211) % 501 for i in range(batch)]
+    lens[-1] = 500
+    q, k, v = _cross_inputs(t + batch, batch, t, 500, *heads)
+    _cross_check(q, _spoil(k, lens), _spoil(v, lens), lens)
+
+
 @pytest.mark.parametrize("t", [1, 150])
 def test_cross_attn_lengths_are_clamped(t):
     q, k, v = _cross_inputs(t + 7, 3, t, 100, 2, 2)
@@ -530,6 +593,32 @@ def test_backward_ragged_sources(t):
     assert not bool(dq[0].any())
     for i, m in enumerate(lens):
         assert not bool(dk[i, m:].any()) and not bool(dv[i, m:].any())
+
+
+@pytest.mark.parametrize("batch,heads", [(12, (16, 8)), (40, (6, 6))], ids=["few entries", "many entries"])
+def test_backward_more_items_than_sms(batch, heads):
+    """Every CTA takes several items, of many and of no tiles."""
+    lens = [(i * 211) % 301 for i in range(batch)]
+    lens[-1] = 300
+    q, k, v = _cross_inputs(batch, batch, 200, 300, *heads)
+    do = _randn(torch.Generator().manual_seed(batch), *q.shape)
+    dq, dk, dv = _grad_check(q, _spoil(k, lens), _spoil(v, lens), do, lens)
+    for i, m in enumerate(lens):
+        assert not bool(dk[i, m:].any()) and not bool(dv[i, m:].any())
+
+
+@pytest.mark.parametrize("shape", [(1, 700, 500, 8, 1), (1, 60, 3500, 4, 2), (2, 1300, 40, 4, 1)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_backward_few_long_items(shape):
+    """Fewer items than SMs, each with many tiles: many query rows per key tile, or many keys per query tile."""
+    b, t, n, h, kv = shape
+    lens = None if b == 1 else [n, n // 3]
+    q, k, v = _cross_inputs(n, b, t, n, h, kv)
+    do = _randn(torch.Generator().manual_seed(t), *q.shape)
+    if lens is not None:
+        k, v = _spoil(k, lens), _spoil(v, lens)
+    first = _grad_check(q, k, v, do, lens)
+    assert all(torch.equal(a, c) for a, c in zip(first, _grad_check(q, k, v, do, lens)))
 
 
 def test_backward_strides_and_scale():
@@ -653,6 +742,34 @@ def test_other_stream_and_captured_graphs():
             _within(outs[i][0], want, bound)
             _within(outs[i][1], *ref.cross_attn(new[i], cross[1], cross[2])["out"])
         assert torch.equal(on_side[0], outs[0][0]) and torch.equal(on_side[1], outs[0][1])
+
+
+def test_calls_on_two_streams_at_once():
+    """Forward, backward and cache calls of two streams beside each other, each as when alone."""
+    g = torch.Generator().manual_seed(51)
+    sets = []
+    for i in range(2):
+        q, k, v = _on(_cross_inputs(52 + i, 2, 300 + 200 * i, 700, 8, 2))
+        cache = _on(_filled(g, [3000, 10 + i, 9000], 1, 64))
+        sets.append((q, k, v, torch.randn_like(q), cache, _randn(g, 3, 1, 8, 128).to(DEV), torch.randn_like(q[:, :1])))
+
+    def run(s, stream):
+        q, k, v, do, cache, dq, few = s
+        out, lse = b200_gemm.cross_attn(q, k, v, return_lse=True, stream=stream)
+        return [out, lse, *b200_gemm.cross_attn_backward(do, q, k, v, out, lse, stream=stream),
+                b200_gemm.cache_attn(dq, *cache, stream=stream), b200_gemm.cross_attn(few, k, v, stream=stream)]
+
+    alone = [run(s, None) for s in sets]
+    _ok()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(sets):
+            got[i].append(run(s, streams[i]))
+    _ok()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(alone[i], r))
 
 
 def test_decoder_layer_steps():
