@@ -123,8 +123,8 @@ _SIGNATURES = {
     "b200_cross_attn_bf16": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, ctypes.c_void_p, _VIEW, ctypes.c_void_p, ctypes.c_int64,
                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                             ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
-    "b200_cross_attn_bwd_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-                                                           ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_cross_attn_bwd_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                                           ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]),
     "b200_cross_attn_bwd_bf16": (ctypes.c_int, [_VIEW, _VIEW, _VIEW, _VIEW, _VIEW, ctypes.c_void_p, ctypes.c_void_p, _VIEW,
                                                 _VIEW, _VIEW, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                 ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,

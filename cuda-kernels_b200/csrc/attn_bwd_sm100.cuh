@@ -21,6 +21,10 @@
 // heads, where an item has 4 to 11 tile pairs and start-up, epilogue and CTA
 // exchange took as long as those.)
 //
+// Where there are fewer gradient tiles than SMs, a tile's walk is cut into parts, items
+// of their own whose fp32 sums attn_bwd_merge_kernel adds in order (one entry, 2048 queries and keys, 8 query and
+// 2 key/value heads: 73 us against 154; 4096 queries, 128 keys, 16 and 2 heads: 58 against 481).
+//
 // One body for both kinds.  X1, X2 are the item's own tiles, Y1, Y2 the
 // streamed ones; rows of the products are X's rows (TMEM lanes), columns Y's:
 //   dK/dV: X = K, V   Y = Q, dO   T1 = S^T, T2 = dP^T;  acc1 (dK) += dS^T Q, acc2 (dV) += P^T dO
@@ -64,6 +68,8 @@ struct AttnBwdParams {
   int32_t q_len, kv_len, heads, kv_heads, group, batch;
   int32_t q_tiles, kv_tiles;
   int32_t items;           // of this kernel's kind
+  int32_t parts;           // items a tile's walk is cut into; their sums are added by attn_bwd_merge_kernel
+  float* part;             // with several parts: [batch, heads, tiles, parts][dK and dV, or dQ][8 warps][16][32] float4
   uint32_t ordered;        // entries by falling number of keys (more items than SMs, at most 32 entries)
   uint32_t early;          // dQ: launched behind the dK/dV kernel, of which it needs nothing
   const int32_t* kv_lens;  // [batch] or NULL
@@ -80,6 +86,11 @@ struct AttnBwdParams {
 struct AttnBwdMaps {
   CUtensorMap q, k, v, dout;
 };
+
+// An item's share of a walk over n tiles: [first, second).
+__host__ __device__ __forceinline__ int bwd_part_begin(int n, int part, int parts) {
+  return (int)((int64_t)n * part / parts);
+}
 
 struct AttnBwdDeltaParams {
   const __nv_bfloat16* o;
@@ -149,8 +160,8 @@ struct AttnBwdPlan {
   static constexpr int kOffOut = kOffVec + (kDQ ? 0 : kY1Stages * 1024);
   static constexpr int kOffBar = kOffOut + (kDQ ? 0 : 8 * 2048);
   static constexpr int kNumBars = 2 + 3 * kY1Stages + 2 * kY2Stages + 2 + 1 + 1 + 1 + 2 + 1 + 1 + 4;
-  static constexpr int kOffItem = kOffBar + kNumBars * 8;  // two slots of (item or -1, keys of its entry)
-  static constexpr int kOffOrder = kOffItem + 16;  // batches of up to 32: the entries by falling number of keys
+  static constexpr int kOffItem = (kOffBar + kNumBars * 8 + 15) / 16 * 16;  // two slots of an Item
+  static constexpr int kOffOrder = kOffItem + 64;  // batches of up to 32: the entries by falling number of keys
   static constexpr int kOffTmemHolder = kOffOrder + 32 * 4;
   static constexpr int kOffAbort = kOffTmemHolder + 4;
   static constexpr int kBytes = kOffAbort + 4;
@@ -276,7 +287,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t drain = bar0 + 8u * (kB + 8);
   auto item_full = [&](uint32_t k) { return bar0 + 8u * (kB + 9 + (k & 1u)); };
   auto item_empty = [&](uint32_t k) { return bar0 + 8u * (kB + 11 + (k & 1u)); };
-  volatile int2* items = reinterpret_cast<volatile int2*>(base_ptr + Plan::kOffItem);
   volatile int32_t* order = reinterpret_cast<volatile int32_t*>(base_ptr + Plan::kOffOrder);
   volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffTmemHolder);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_ptr + Plan::kOffAbort);
@@ -337,26 +347,45 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     __syncthreads();
   }
 
-  // An item: its tile, head and entry, and the number of tiles to stream.
+  // An item, worked out by the producer and read by the others from shared memory.
   // Entries with many keys come first, so that the last items are short.  Tiles
   // change fastest: neighbours stream the same tiles.  (Entries fastest, so
   // that long and short ones alternate: 4 % slower on 8 ragged pairs.)
-  struct Item {
-    int tile, head, bat, kv_len, n;
-    bool clean;  // dQ: rows of the last K tile past the last key, which TMA filled from memory
+  struct alignas(16) Item {
+    int tile, part, head, bat;
+    int i0, n;   // the tiles of its walk
+    int kv_len;  // keys of its entry
+    int flags;   // 1: no item, the end; 2: dQ, the last K tile has rows past the last key, which TMA filled from memory
+    __device__ bool clean() const { return (flags & 2) != 0; }
   };
-  auto item_of = [&](int id, int kv_len) {
+  static_assert(sizeof(Item) == 32, "two 16-byte words of shared memory");
+  auto item_at = [&](uint32_t k) { return reinterpret_cast<int4*>(base_ptr + Plan::kOffItem + (k & 1u) * 32u); };
+  auto item_of = [&](int id) {
     const int tiles = kDQ ? p.q_tiles : p.kv_tiles, heads = kDQ ? p.heads : p.kv_heads;
-    Item t;
+    Item t{};
+    if (id >= p.items) {
+      t.flags = 1;
+      return t;
+    }
     t.tile = id % tiles;
-    t.head = (id / tiles) % heads;
-    t.bat = (id / tiles) / heads;
+    id /= tiles;
+    t.part = id % p.parts;
+    id /= p.parts;
+    t.head = id % heads;
+    t.bat = id / heads;
     if (p.ordered) t.bat = order[t.bat];
-    t.kv_len = kv_len;
-    const int kv_tiles = (kv_len + 127) / 128;
-    t.n = kDQ ? kv_tiles : (t.tile < kv_tiles ? p.group * p.q_tiles : 0);
-    t.clean = kDQ && kv_len < p.kv_len && kv_len % 128 != 0;
+    t.kv_len = attn_kv_len(p.kv_lens, t.bat, p.kv_len);
+    const int kv_tiles = (t.kv_len + 127) / 128;
+    const int walk = kDQ ? kv_tiles : (t.tile < kv_tiles ? p.group * p.q_tiles : 0);
+    t.i0 = bwd_part_begin(walk, t.part, p.parts);
+    t.n = bwd_part_begin(walk, t.part + 1, p.parts) - t.i0;
+    if (kDQ && t.i0 + t.n == walk && t.kv_len < p.kv_len && t.kv_len % 128 != 0) t.flags = 2;
     return t;
+  };
+  auto read_item = [&](uint32_t k, Item* t) {
+    const int4 a = item_at(k)[0], b = item_at(k)[1];
+    t->tile = a.x, t->part = a.y, t->head = a.z, t->bat = a.w;
+    t->i0 = b.x, t->n = b.y, t->kv_len = b.z, t->flags = b.w;
   };
   // The k-th item of this CTA, for one reader (a warp, or the MMA lane); false at the end.
   auto next_item = [&](uint32_t k, bool whole_warp, Item* t, bool* ok) {
@@ -366,12 +395,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       *ok = false;
       return false;
     }
-    const int id = items[k & 1u].x, kv_len = items[k & 1u].y;
+    read_item(k, t);
     if (whole_warp) __syncwarp();
     if (!whole_warp || lane == 0) mbar_arrive(item_empty(k));
-    if (id < 0) return false;
-    *t = item_of(id, kv_len);
-    return true;
+    return (t->flags & 1) == 0;
   };
   // TMEM regions of T1 and T2 of tile pair g (see the head of the file).
   auto reg1 = [&](uint32_t g) { return tmem_base + (kDQ ? ((g & 1u) ? 384u : 0u) : ((g & 1u) ? 128u : 0u)); };
@@ -396,15 +423,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             ok = false;
             break;
           }
-          const bool end = id >= p.items;
-          int bat = end ? 0 : id / (kDQ ? p.q_tiles * p.heads : p.kv_tiles * p.kv_heads);
-          if (p.ordered) bat = order[bat];
-          const int kv_len = end ? 0 : attn_kv_len(p.kv_lens, bat, p.kv_len);
-          items[k & 1u].x = end ? -1 : id;
-          items[k & 1u].y = kv_len;
+          const Item t = item_of(id);
+          item_at(k)[0] = make_int4(t.tile, t.part, t.head, t.bat);
+          item_at(k)[1] = make_int4(t.i0, t.n, t.kv_len, t.flags);
           mbar_arrive(item_full(k));
-          if (end) break;
-          const Item t = item_of(id, kv_len);
+          if (t.flags & 1) break;
           id = (int)(gridDim.x + atomicAdd(p.counter, 1u));  // the next one
           if (t.n == 0) continue;
           auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int h, int row, uint64_t pol) {
@@ -418,14 +441,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           load(sX1, kDQ ? &tm.q : &tm.k, x_full, t.head, t.tile * 128, pol_once);
           load(sX2, kDQ ? &tm.dout : &tm.v, x_full, t.head, t.tile * 128, pol_once);
           ++filled;
-          for (int i = 0; i < t.n; ++i) {
+          for (int i = t.i0; i < t.i0 + t.n; ++i) {
             const int y_head = kDQ ? t.head / p.group : t.head * p.group + i / p.q_tiles;
             const int y_row = (kDQ ? i : i % p.q_tiles) * 128;
             if (!mbar_wait(y1_empty(g), y1_par(g) ^ 1u, p.timeout_ns, abort_flag)) {
               ok = false;
               break;
             }
-            raw_last = t.clean && i == t.n - 1;
+            raw_last = t.clean() && i == t.i0 + t.n - 1;
             const uint32_t y1_bar = raw_last ? y1_raw(g) : y1_full(g);
             mbar_arrive_expect_tx(y1_bar, Plan::kTileBytes + (kDQ ? 0 : 1024));
             load(sY1(g), kDQ ? &tm.k : &tm.q, y1_bar, y_head, y_row, pol_keep);
@@ -559,12 +582,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (uint32_t k = 0;; ++k) {
         ok = both(mbar_wait(item_full(k), (k >> 1) & 1u, p.timeout_ns, abort_flag));
         if (!ok) break;
-        const int id = items[k & 1u].x, kv_len = items[k & 1u].y;
+        Item t;
+        read_item(k, &t);
         __syncwarp();
         if (lane == 0) mbar_arrive(item_empty(k));
-        if (id < 0) break;
-        const Item t = item_of(id, kv_len);
+        if (t.flags & 1) break;
         if (t.n == 0) {
+          if (p.parts > 1) continue;  // (the merge knows)
 #pragma unroll 1
           for (int part = warp - kAttnMmaWarp - 1; part < 8; part += 2) {  // 32 rows x 64 columns
             const int row0 = t.tile * 128 + (part >> 1) * 32, rows = kDQ ? p.q_len : p.kv_len, col = (part & 1) * 64;
@@ -574,12 +598,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           continue;
         }
         g += (uint32_t)t.n;
-        if (!t.clean) continue;
+        if (!t.clean()) continue;
         const uint32_t last = g - 1;
         ok = both(mbar_wait(y1_raw(last), (raw_par >> (last % S1)) & 1u, p.timeout_ns, abort_flag));
         if (!ok) break;
         raw_par ^= 1u << (last % S1);
-        const int cells = (128 * t.n - t.kv_len) * 16;  // 16-byte cells, both 64-column atoms
+        const int cells = (128 * (t.i0 + t.n) - t.kv_len) * 16;  // 16-byte cells, both 64-column atoms
         for (int c = (warp - kAttnMmaWarp - 1) * 32 + (int)lane; c < cells; c += 64) {
           const uint32_t dst = sY1(last) + (uint32_t)(((c >> 3) & 1) * 16384 + (127 - (c >> 4)) * 128 + (c & 7) * 16);
           asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
@@ -615,6 +639,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (uint32_t k = 0; ok && next_item(k, true, &t, &ok); ++k) {
       const int kv_len = t.kv_len, n = t.n;
       if (n == 0) continue;
+      const int kv_left = kv_len - t.i0 * 128;  // dQ: keys from the item's first tile on
       float row_lse = 0.0f, row_delta = 0.0f;  // dQ: of this thread's query row
       if constexpr (kDQ) {
         const size_t at = ((size_t)t.bat * p.heads + t.head) * (size_t)(p.q_tiles * 128) + t.tile * 128 + row;
@@ -654,8 +679,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           e[c + 2] = fast_exp2(b.x);
           e[c + 3] = fast_exp2(b.y);
         }
-        if (kDQ && i == n - 1 && n * 128 > kv_len) {
-          const int lim = kv_len - i * 128 - wg * 64;
+        if (kDQ && i == n - 1 && n * 128 > kv_left) {
+          const int lim = kv_left - i * 128 - wg * 64;
 #pragma unroll
           for (int c = 0; c < 64; ++c) e[c] = c < lim ? e[c] : 0.0f;
         }
@@ -694,8 +719,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
         // 0 x (NaN - delta): masked places again, on the packed pairs.
-        if (kDQ && i == n - 1 && n * 128 > kv_len) {
-          const int lim = kv_len - i * 128 - wg * 64;
+        if (kDQ && i == n - 1 && n * 128 > kv_left) {
+          const int lim = kv_left - i * 128 - wg * 64;
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             dw[c] &= (2 * c < lim ? 0xffffu : 0u) | (2 * c + 1 < lim ? 0xffff0000u : 0u);
@@ -728,6 +753,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int c = 0; c < 32; ++c) lo[c] = hi[c] = 0u;
         }
+        if (p.parts > 1) {
+          const int tiles = kDQ ? p.q_tiles : p.kv_tiles, heads = kDQ ? p.heads : p.kv_heads;
+          const int64_t slot = (((int64_t)t.bat * heads + t.head) * tiles + t.tile) * p.parts + t.part;
+          float4* dst = reinterpret_cast<float4*>(p.part) + ((slot * (kDQ ? 1 : 2) + h) * 8 + warp) * 512 + lane;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            dst[c * 32] = make_float4(__uint_as_float(lo[4 * c]), __uint_as_float(lo[4 * c + 1]), __uint_as_float(lo[4 * c + 2]),
+                                      __uint_as_float(lo[4 * c + 3]));
+            dst[(c + 8) * 32] = make_float4(__uint_as_float(hi[4 * c]), __uint_as_float(hi[4 * c + 1]),
+                                            __uint_as_float(hi[4 * c + 2]), __uint_as_float(hi[4 * c + 3]));
+          }
+          continue;
+        }
         store_grad<kDQ>(grad, t.bat, t.tile * 128 + qw * 32, rows, t.head, wg * 64, lane, lo, hi, h == 0 ? p.scale : 1.0f,
                         base + (uint32_t)(Plan::kOffOut + warp * 2048));
       }
@@ -747,6 +785,70 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   // Started early: what follows this kernel must find the dK/dV kernel complete too.
   if (kDQ && p.early != 0u) pdl_wait();
 #endif  // B200_NO_SM100A_FEATURES
+}
+
+struct AttnBwdMergeParams {
+  // Of dK and dV (0) and of dQ (1): parts 1 means the gradients are there already.
+  const float* part[2];
+  int32_t parts[2], tiles[2], heads[2];
+  int32_t blocks;          // of dK and dV
+  int32_t q_len, kv_len, walk;  // walk: tile pairs of a dK/dV tile
+  const int32_t* kv_lens;
+  AttnGrad dq, dk, dv;
+  float scale;
+};
+
+// Adds the parts of each gradient tile in order.  A thread has 8 columns of a
+// row, 8 lanes a row's 64 columns, a block 16 rows of one tile: loads in runs
+// of 64 bytes, stores of 128.
+__global__ void __launch_bounds__(256) attn_bwd_merge_kernel(const __grid_constant__ AttnBwdMergeParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int kind = (int)blockIdx.x < p.blocks ? 0 : 1;
+  int64_t id = kind == 0 ? blockIdx.x : blockIdx.x - p.blocks;
+  const int slice = (int)(id & 7);
+  id >>= 3;
+  const int grads = kind == 0 ? 2 : 1;
+  const int h = (int)(id % grads);
+  const int64_t slot = id / grads;
+  const int tile = (int)(slot % p.tiles[kind]), head = (int)(slot / p.tiles[kind] % p.heads[kind]);
+  const int bat = (int)(slot / p.tiles[kind] / p.heads[kind]);
+  const int lane = (int)(threadIdx.x & 31u), warp = (int)(threadIdx.x >> 5);
+  // Of the tile: four rows a warp, 64 columns of its computing warp.
+  const int r = slice * 16 + (warp & 3) * 4 + (lane & 3), c = lane >> 2, wg = warp >> 2;
+  const int kv_len = attn_kv_len(p.kv_lens, bat, p.kv_len), kv_tiles = (kv_len + 127) / 128;
+  const int walk = kind == 1 ? kv_tiles : (tile < kv_tiles ? p.walk : 0);
+  const int parts = p.parts[kind];
+  const float4* src = reinterpret_cast<const float4*>(p.part[kind]) + (slot * parts * grads + h) * 4096 +
+                      (wg * 4 + (r >> 5)) * 512 + c * 64 + (r & 31);
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+  for (int s0 = 0; s0 < parts; s0 += 4) {
+    float4 x[4], y[4];
+    bool has[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i;
+      has[i] = s < parts && bwd_part_begin(walk, s, parts) < bwd_part_begin(walk, s + 1, parts);  // else not written
+      x[i] = y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (has[i]) {
+        x[i] = src[(int64_t)s * grads * 4096];
+        y[i] = src[(int64_t)s * grads * 4096 + 32];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a.x += x[i].x, a.y += x[i].y, a.z += x[i].z, a.w += x[i].w;
+      b.x += y[i].x, b.y += y[i].y, b.z += y[i].z, b.w += y[i].w;
+    }
+  }
+  const AttnGrad& g = kind == 1 ? p.dq : (h == 0 ? p.dk : p.dv);
+  const float f = h == 0 ? p.scale : 1.0f;
+  const int row = tile * 128 + r;
+  if (row < (kind == 1 ? p.q_len : p.kv_len)) {
+    *reinterpret_cast<uint4*>(g.data + bat * g.batch_stride + row * g.seq_stride + head * g.head_stride + wg * 64 + c * 8) =
+        make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f), pack_bf16x2(b.x * f, b.y * f),
+                   pack_bf16x2(b.z * f, b.w * f));
+  }
 }
 
 }  // namespace b200

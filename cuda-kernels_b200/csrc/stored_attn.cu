@@ -596,14 +596,77 @@ int64_t bwd_padded(int64_t q_len) { return (q_len + 127) / 128 * 128; }
 size_t bwd_bytes(int64_t batch, int64_t q_len, int64_t heads) {
   return kWsAlign + 2 * sizeof(float) * (size_t)(batch * heads) * (size_t)bwd_padded(q_len);
 }
+
+// Work items of the two backward kernels: dK/dV (0) and dQ (1).
+struct BwdShape {
+  int64_t tiles[2], items[2];  // gradient tiles per head, and of all heads and entries
+  int64_t walk[2];             // tile pairs per gradient tile, at most
+  int parts[2];                // items per gradient tile
+  size_t part_floats(int kind) const {
+    return parts[kind] > 1 ? (size_t)(items[kind] * parts[kind]) * (kind == 0 ? 2 : 1) * 128 * 128 : 0;
+  }
+  size_t part_bytes() const { return (part_floats(0) + part_floats(1)) * sizeof(float); }
+};
+
+int check_bwd_size(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads) {
+  if (kv_len > kLim - 128 || q_len > kLim - 128) return B200_ERR_TOO_LARGE;
+  const int64_t q_tiles = (q_len + 127) / 128, kv_tiles = (kv_len + 127) / 128;
+  const int64_t dkv = kv_tiles * kv_heads, dq = q_tiles * heads;  // (below 2^41)
+  if (dq > kLim || (double)batch * (double)(dkv + dq) > (double)kLim) return B200_ERR_TOO_LARGE;
+  return B200_OK;
+}
+
+BwdShape plan_bwd(int sm_count, int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads) {
+  const int64_t q_tiles = heads > 0 ? (q_len + 127) / 128 : 0, kv_tiles = kv_heads > 0 ? (kv_len + 127) / 128 : 0;
+  BwdShape s{};
+  s.tiles[0] = kv_tiles, s.tiles[1] = q_tiles;
+  s.items[0] = kv_tiles * kv_heads * batch, s.items[1] = q_tiles * heads * batch;
+  s.walk[0] = kv_heads > 0 ? heads / kv_heads * q_tiles : 0, s.walk[1] = kv_tiles;
+  s.parts[0] = s.parts[1] = 1;
+  if (s.items[0] == 0 || s.items[1] == 0) return s;
+  // With fewer gradient tiles than SMs the longest item is most of the time; its
+  // walk is cut where the sums' way through memory and another kernel cost less.
+  // On a B200: 2.0 (dK/dV) and 1.5 us (dQ) a tile pair and 4 an item, all items
+  // on all SMs plus half of the longest; the sums 64 KiB a tile and part out and
+  // back at 4 TB/s, and 4 us for their kernel.
+  constexpr double kPair[2] = {2.0, 1.5};
+  constexpr int kTry[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  double best = 0.0;
+  int64_t most[2];
+  for (int k = 0; k < 2; ++k) most[k] = s.items[k] < sm_count ? std::min(s.walk[k] / 2, 2 * (sm_count / s.items[k])) : 1;
+  for (const int a : kTry) {
+    if (a > 1 && a > most[0]) break;
+    for (const int b : kTry) {
+      if (b > 1 && b > most[1]) break;
+      const int parts[2] = {a, b};
+      double all = 0.0, longest = 0.0, floats = 0.0;
+      for (int k = 0; k < 2; ++k) {
+        all += (double)s.items[k] * (4.0 * parts[k] + kPair[k] * (double)s.walk[k]) / sm_count;
+        longest = std::max(longest, 4.0 + kPair[k] * (double)((s.walk[k] + parts[k] - 1) / parts[k]));
+        if (parts[k] > 1) floats += (double)(s.items[k] * parts[k]) * (k == 0 ? 2 : 1) * 128 * 128;
+      }
+      const double t = std::max(longest, all + 0.5 * longest) + (floats > 0.0 ? 4.0 + 8.0 * floats / 4e6 : 0.0);
+      if (best == 0.0 || t < best) {
+        best = t;
+        s.parts[0] = a, s.parts[1] = b;
+      }
+    }
+  }
+  return s;
+}
 }  // namespace
 
-extern "C" B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t heads, size_t* bytes) {
+extern "C" B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
+                                                            int64_t kv_heads, size_t* bytes) {
   if (bytes == nullptr) return B200_ERR_INVALID_ARG;
   *bytes = 0;
-  const int rc = check_heads(batch, q_len, heads, heads, b200::kKvD);
+  int rc = check_heads(batch, q_len, heads, kv_heads, b200::kKvD);
   if (rc != B200_OK) return rc;
-  *bytes = bwd_bytes(batch, q_len, heads);
+  if (kv_len < 0) return B200_ERR_INVALID_ARG;
+  if ((rc = check_bwd_size(batch, q_len, kv_len, heads, kv_heads)) != B200_OK) return rc;
+  b200::DeviceInfo di;
+  if ((rc = b200::device_info(&di)) != B200_OK) return rc;
+  *bytes = bwd_bytes(batch, q_len, heads) + plan_bwd(di.sm_count, batch, q_len, kv_len, heads, kv_heads).part_bytes();
   return B200_OK;
 }
 
@@ -619,11 +682,8 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   if (kv_len < 0 || !scale_ok(scale)) return B200_ERR_INVALID_ARG;
   const bool queries = q_len > 0 && heads > 0, keys = kv_len > 0 && kv_heads > 0;
   if (batch == 0 || (!queries && !keys)) return B200_OK;
+  if ((rc = check_bwd_size(batch, q_len, kv_len, heads, kv_heads)) != B200_OK) return rc;
   const int64_t q_tiles = queries ? (q_len + 127) / 128 : 0, kv_tiles = keys ? (kv_len + 127) / 128 : 0;
-  const int64_t dkv_items = kv_tiles * kv_heads * batch, dq_items = q_tiles * heads * batch;
-  if (kv_len > kLim - 128 || q_len > kLim - 128 || dkv_items > kLim || dq_items > kLim - dkv_items ||
-      q_tiles * std::max<int64_t>(heads, 1) > kLim)
-    return B200_ERR_TOO_LARGE;
   b200_attn_view qq{}, oo{}, dd{}, dqv{}, kk{}, vv{}, dkv{}, dvv{};
   if (queries) {
     if ((rc = check_view(q, batch, q_len, heads, &qq)) != B200_OK || (rc = check_view(o, batch, q_len, heads, &oo)) != B200_OK ||
@@ -644,6 +704,9 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   StoredState* st = nullptr;
   if ((rc = current_state(&di, &st)) != B200_OK) return rc;
   if (!st->bwd_regs_ok) return B200_ERR_CUDA;  // built with another register count: never launch it
+  const BwdShape shape = plan_bwd(di.sm_count, batch, q_len, kv_len, heads, kv_heads);
+  const size_t sums = bwd_bytes(batch, q_len, heads);  // where the parts' sums begin
+  if (workspace_bytes < sums + shape.part_bytes()) return B200_ERR_INVALID_ARG;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   b200::AttnBwdMaps tm{};
   if (queries && ((rc = encode_view(di, &tm.q, qq, batch, q_len, heads, 128, true)) != B200_OK ||
@@ -693,24 +756,41 @@ extern "C" B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const 
   const dim3 grid((unsigned)std::max<int64_t>(q_tiles * 2, 1), (unsigned)std::min<int64_t>(rows, 65535),
                   (unsigned)((rows + 65534) / 65535));
   if ((rc = launch(b200::attn_bwd_delta_kernel, grid, 256, 0, stream, d)) != B200_OK) return rc;
-  auto order = [&](int64_t items) {
-    return kv_lens != nullptr && batch > 1 && batch <= 32 && items > di.sm_count ? 1u : 0u;
-  };
-  if (dkv_items > 0) {
-    p.items = (int32_t)dkv_items;
-    p.ordered = order(dkv_items);
-    p.counter = counters;
-    if ((rc = launch(b200::attn_bwd_kernel<false>, dim3((unsigned)std::min<int64_t>(dkv_items, di.sm_count)),
-                     b200::kAttnThreads, b200::AttnBwdPlan<false>::kAllocBytes, stream, tm, p)) != B200_OK)
-      return rc;
+  float* part[2];
+  part[0] = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums);
+  part[1] = part[0] + shape.part_floats(0);
+  for (int kind = 0; kind < 2; ++kind) {
+    const int64_t items = shape.items[kind] * shape.parts[kind];
+    if (items == 0) continue;
+    p.items = (int32_t)items;
+    p.parts = shape.parts[kind];
+    p.part = part[kind];
+    p.ordered = kv_lens != nullptr && batch > 1 && batch <= 32 && items > di.sm_count ? 1u : 0u;
+    p.counter = counters + kind;
+    p.early = kind == 1 && shape.items[0] > 0 ? 1u : 0u;
+    const dim3 ctas((unsigned)std::min<int64_t>(items, di.sm_count));
+    rc = kind == 0 ? launch(b200::attn_bwd_kernel<false>, ctas, b200::kAttnThreads, b200::AttnBwdPlan<false>::kAllocBytes,
+                            stream, tm, p)
+                   : launch(b200::attn_bwd_kernel<true>, ctas, b200::kAttnThreads, b200::AttnBwdPlan<true>::kAllocBytes,
+                            stream, tm, p);
+    if (rc != B200_OK) return rc;
   }
-  if (dq_items > 0) {
-    p.items = (int32_t)dq_items;
-    p.ordered = order(dq_items);
-    p.counter = counters + 1;
-    p.early = dkv_items > 0 ? 1u : 0u;
-    rc = launch(b200::attn_bwd_kernel<true>, dim3((unsigned)std::min<int64_t>(dq_items, di.sm_count)), b200::kAttnThreads,
-                b200::AttnBwdPlan<true>::kAllocBytes, stream, tm, p);
+  if (shape.part_bytes() == 0) return B200_OK;
+  b200::AttnBwdMergeParams m{};
+  int blocks[2];
+  for (int kind = 0; kind < 2; ++kind) {
+    m.part[kind] = part[kind];
+    m.parts[kind] = shape.parts[kind];
+    m.tiles[kind] = (int32_t)shape.tiles[kind];
+    m.heads[kind] = kind == 0 ? p.kv_heads : p.heads;
+    blocks[kind] = shape.parts[kind] > 1 ? (int)shape.items[kind] * (kind == 0 ? 2 : 1) * 8 : 0;
   }
-  return rc;
+  m.blocks = blocks[0];
+  m.q_len = p.q_len;
+  m.kv_len = p.kv_len;
+  m.walk = (int32_t)shape.walk[0];
+  m.kv_lens = kv_lens;
+  m.dq = p.dq, m.dk = p.dk, m.dv = p.dv;
+  m.scale = scale;
+  return launch(b200::attn_bwd_merge_kernel, dim3((unsigned)(blocks[0] + blocks[1])), 256, 0, stream, m);
 }

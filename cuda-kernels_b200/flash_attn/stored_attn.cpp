@@ -276,7 +276,7 @@ std::tuple<Tensor, Tensor, Tensor> cross_attn_backward(const Tensor& dout, const
                dv = scope.empty(v.sizes(), torch::kBFloat16);
   const b200_attn_view dqv = view_of("dq", dq), dkv = view_of("dk", dk), dvv = view_of("dv", dv);
   size_t bytes = 0;
-  int rc = b200_cross_attn_bwd_workspace_bytes(s.batch, s.q_len, s.heads, &bytes);
+  int rc = b200_cross_attn_bwd_workspace_bytes(s.batch, s.q_len, s.kv_len, s.heads, s.kv_heads, &bytes);
   if (rc == B200_OK) {
     const Tensor ws = scope.workspace(bytes);
     rc = b200_cross_attn_bwd_bf16(&qq, &kk, &vv, &oo, &dd, static_cast<const float*>(lse.data_ptr()), lens, &dqv, &dkv, &dvv,

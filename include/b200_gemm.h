@@ -359,7 +359,8 @@ B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200_attn_view*
  * b200_cross_attn_bwd_workspace_bytes, as above.  No reference counterpart
  * (the reference has no backward pass).
  */
-B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t heads, size_t* bytes);
+B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
+                                                 int64_t kv_heads, size_t* bytes);
 B200_API int b200_cross_attn_bwd_bf16(const b200_attn_view* q, const b200_attn_view* k, const b200_attn_view* v,
                                       const b200_attn_view* o, const b200_attn_view* dout, const float* lse,
                                       const int32_t* kv_lens, const b200_attn_view* dq, const b200_attn_view* dk,

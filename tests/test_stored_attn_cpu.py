@@ -134,9 +134,10 @@ def test_cross_attn_backward_refusals():
     assert call(batch=0) == _lib.B200_OK
     assert call(q_len=0, kv_len=0) == _lib.B200_OK
     n = ctypes.c_size_t(0)
-    assert lib.b200_cross_attn_bwd_workspace_bytes(2, 129, 4, ctypes.byref(n)) == _lib.B200_OK
-    assert n.value == 256 + 2 * 4 * 8 * 256  # item counters, and two floats per query row of whole tiles
-    assert lib.b200_cross_attn_bwd_workspace_bytes(2, -1, 4, ctypes.byref(n)) == bad
+    assert lib.b200_cross_attn_bwd_workspace_bytes(2, -1, 5, 4, 2, ctypes.byref(n)) == bad
+    assert lib.b200_cross_attn_bwd_workspace_bytes(2, 5, -1, 4, 2, ctypes.byref(n)) == bad
+    assert lib.b200_cross_attn_bwd_workspace_bytes(2, 5, 5, 4, 3, ctypes.byref(n)) == bad
+    assert lib.b200_cross_attn_bwd_workspace_bytes(2, 5, 1 << 31, 4, 2, ctypes.byref(n)) == _lib.B200_ERR_TOO_LARGE
 
 
 def test_status_text():

@@ -607,12 +607,13 @@ def test_backward_more_items_than_sms(batch, heads):
         assert not bool(dk[i, m:].any()) and not bool(dv[i, m:].any())
 
 
-@pytest.mark.parametrize("shape", [(1, 700, 500, 8, 1), (1, 60, 3500, 4, 2), (2, 1300, 40, 4, 1)],
+@pytest.mark.parametrize("shape", [(1, 700, 500, 8, 1), (1, 60, 3500, 4, 2), (2, 1300, 40, 4, 1), (3, 200, 5000, 4, 2),
+                                   (3, 500, 1100, 12, 1), (1, 1, 2000, 8, 2), (4, 2000, 1, 2, 1)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_backward_few_long_items(shape):
     """Fewer items than SMs, each with many tiles: many query rows per key tile, or many keys per query tile."""
     b, t, n, h, kv = shape
-    lens = None if b == 1 else [n, n // 3]
+    lens = None if b == 1 else [n, n // 3, 1, 0][:b]
     q, k, v = _cross_inputs(n, b, t, n, h, kv)
     do = _randn(torch.Generator().manual_seed(t), *q.shape)
     if lens is not None:
