@@ -296,8 +296,8 @@ typedef struct b200_kv_cache {
  * grows, the codes already in the page are rounded to the new scale; a page
  * whose slot 0 is written starts afresh.  Slots behind the new tokens are left
  * as they are.  NaN stays NaN and takes no part in a scale, an infinity
- * counts as bf16's largest value and becomes the largest code.  No page may belong to two sequences that are written in
- * one call.  A sequence whose lengths or pages are out of range is not written
+ * counts as bf16's largest value and becomes the largest code.  No page may
+ * belong to two sequences that are written in one call.  A sequence whose lengths or pages are out of range is not written
  * and is reported by b200_gemm_status (B200_ERR_BAD_INDEX).  Asynchronous; no
  * allocation.  No reference counterpart (the reference's attention has no
  * cache).
@@ -337,10 +337,13 @@ B200_API int b200_cache_attn(const b200_attn_view* q, const b200_kv_cache* cache
  * clamped to [0, kv_len]; what k and v hold behind them is not used.
  * An entry without keys gets O = 0 and lse = -inf.  lse (fp32, [batch, heads,
  * q_len], or NULL): natural log of the softmax denominator, which
- * b200_cross_attn_bwd_bf16 needs.  scale > 0.  Few query rows per key/value
- * head run split along the keys, others on the tcgen05 kernel of
- * b200_flash_attn_bf16.  The workspace (b200_cross_attn_workspace_bytes, 0 for
- * many) as in b200_cache_attn.  o may not overlap an input.  No reference
+ * b200_cross_attn_bwd_bf16 needs.  scale > 0.  Up to 16 query rows per
+ * key/value head run split along the keys (in thread-block clusters, or all keys as one
+ * line over the GPU's warps), others on the tcgen05 kernel of
+ * b200_flash_attn_bf16, in parts along the keys where its grid would leave SMs
+ * idle; the choice is by estimated time from the sizes given here, never from
+ * what is on the device.  The workspace (b200_cross_attn_workspace_bytes, 0 for
+ * many sizes) as in b200_cache_attn.  o may not overlap an input.  No reference
  * counterpart (its operator has one length for queries and keys).
  */
 B200_API int b200_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
@@ -356,7 +359,9 @@ B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200_attn_view*
  * query heads of a group, and 0 behind the keys of an entry.  bf16 operands
  * and results, fp32 sums in a fixed order (no atomics).  The gradients may not
  * overlap an input or each other.  Workspace:
- * b200_cross_attn_bwd_workspace_bytes, as above.  No reference counterpart
+ * b200_cross_attn_bwd_workspace_bytes, as above: 8 bytes per query row and
+ * head, and, where there are fewer 128-row gradient tiles than SMs, up to
+ * about 40 MB of fp32 sums.  No reference counterpart
  * (the reference has no backward pass).
  */
 B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
@@ -434,7 +439,9 @@ B200_API int b200_gemm_bf16_noalloc(const void* A, const void* B, void* C, int64
 /*
  * Waits for `stream`, then reads and clears the current device's status word.
  * Returns B200_OK, B200_ERR_DEVICE_TIMEOUT (a kernel gave up on a wait; the
- * raw bits are stored to *device_bits if non-NULL), or B200_ERR_CUDA.
+ * raw bits are stored to *device_bits if non-NULL), B200_ERR_BAD_INDEX (only
+ * that: a length or page of the key/value cache was out of range), or
+ * B200_ERR_CUDA.
  * The reference has no error reporting at all (host assert only,
  * bf16_matmul/matmul_v8_tuned.cu:238).
  */

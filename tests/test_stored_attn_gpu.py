@@ -516,6 +516,19 @@ def test_cross_attn_growing_scores():
         _cross_check(q, k, v)
 
 
+@pytest.mark.parametrize("t", [1, 130])
+@pytest.mark.parametrize("n", [1, 64, 128, 1000])
+def test_cross_attn_lse_of_equal_keys(t, n):
+    """q = 0: every key weighs exactly 1 and the sum is n; log2, its product with ln 2 and the parts' weights add less than
+    2^-20 (1 + lse)."""
+    q, k, v = _cross_inputs(t + n, 1, t, n, 2, 2)
+    q.zero_()
+    out, lse = b200_gemm.cross_attn(*_on([q, k, v]), return_lse=True)
+    _ok()
+    assert float((lse.double().cpu() - math.log(n)).abs().max()) <= 2.0 ** -20 * (1 + math.log(n))
+    _within(out, *ref.cross_attn(q, k, v)["out"])
+
+
 def test_cross_attn_agrees_with_flash_attn_on_square_shapes():
     """The same function: both within the bound of the exact result (their key tiles may be added in another order)."""
     for n in (384, 512):
