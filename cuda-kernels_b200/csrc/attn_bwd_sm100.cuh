@@ -23,7 +23,7 @@
 //
 // Where there are fewer gradient tiles than SMs, a tile's walk is cut into parts, items
 // of their own whose fp32 sums attn_bwd_merge_kernel adds in order (one entry, 2048 queries and keys, 8 query and
-// 2 key/value heads: 73 us against 154; 4096 queries, 128 keys, 16 and 2 heads: 58 against 481).
+// 2 key/value heads: 73 us against 154; 4096 queries, 128 keys, 16 and 2 heads: 57 against 481).
 //
 // One body for both kinds.  X1, X2 are the item's own tiles, Y1, Y2 the
 // streamed ones; rows of the products are X's rows (TMEM lanes), columns Y's:

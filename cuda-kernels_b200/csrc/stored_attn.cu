@@ -616,6 +616,29 @@ int check_bwd_size(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads, 
   return B200_OK;
 }
 
+// When n0 items of time t0, and behind them n1 of time t1, have run on sms SMs.
+double bwd_end(int sms, int64_t n0, double t0, int64_t n1, double t1) {
+  const int64_t late = n0 % sms;  // SMs that have one item more of the first kind
+  const double free[2] = {(double)(n0 / sms) * t0, (double)(n0 / sms + (late > 0)) * t0};
+  const int64_t on[2] = {sms - late, late};
+  // All SMs busy to the end is the least; from there, to where the items fit.
+  const double least = ((double)n0 * t0 + (double)n1 * t1) / sms;
+  double done[2], end = free[1];
+  int64_t left = n1;
+  for (int i = 0; i < 2; ++i) {
+    done[i] = std::max(0.0, std::floor((least - free[i]) / t1));
+    left -= (int64_t)done[i] * on[i];
+  }
+  while (left > 0) {
+    const int i = on[1] > 0 && free[1] + (done[1] + 1.0) * t1 < free[0] + (done[0] + 1.0) * t1 ? 1 : 0;
+    done[i] += 1.0;
+    left -= on[i];
+    end = std::max(end, free[i] + done[i] * t1);
+  }
+  for (int i = 0; i < 2; ++i) end = std::max(end, on[i] > 0 && done[i] > 0.0 ? free[i] + done[i] * t1 : 0.0);
+  return end;
+}
+
 BwdShape plan_bwd(int sm_count, int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads) {
   const int64_t q_tiles = heads > 0 ? (q_len + 127) / 128 : 0, kv_tiles = kv_heads > 0 ? (kv_len + 127) / 128 : 0;
   BwdShape s{};
@@ -626,10 +649,13 @@ BwdShape plan_bwd(int sm_count, int64_t batch, int64_t q_len, int64_t kv_len, in
   if (s.items[0] == 0 || s.items[1] == 0) return s;
   // With fewer gradient tiles than SMs the longest item is most of the time; its
   // walk is cut where the sums' way through memory and another kernel cost less.
-  // On a B200: 2.0 (dK/dV) and 1.5 us (dQ) a tile pair and 4 an item, all items
-  // on all SMs plus half of the longest; the sums 64 KiB a tile and part out and
-  // back at 4 TB/s, and 4 us for their kernel.
-  constexpr double kPair[2] = {2.0, 1.5};
+  // On a B200: 2.3 (dK/dV, with dQ beside it) and 1.5 us (dQ) a tile pair and 4 an
+  // item, dQ items on SMs as they run out of dK/dV items (bwd_end); the sums' kernel 3 us,
+  // and they go 64 KiB a tile and part out and back, mostly through L2, at 12
+  // TB/s.  Measured, dK/dV walks in 1, 2, 3, 4, 6 and 8 parts: 2048 queries and
+  // keys, 8 and 2 heads 154, 100, 83, 75, 88, 81 us; 1024 queries, 256 keys, 32 and 8
+  // heads 79, 53, 45, 40, 40, 39.
+  constexpr double kPair[2] = {2.3, 1.5};
   constexpr int kTry[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
   double best = 0.0;
   int64_t most[2];
@@ -639,13 +665,13 @@ BwdShape plan_bwd(int sm_count, int64_t batch, int64_t q_len, int64_t kv_len, in
     for (const int b : kTry) {
       if (b > 1 && b > most[1]) break;
       const int parts[2] = {a, b};
-      double all = 0.0, longest = 0.0, floats = 0.0;
+      double item[2], floats = 0.0;
       for (int k = 0; k < 2; ++k) {
-        all += (double)s.items[k] * (4.0 * parts[k] + kPair[k] * (double)s.walk[k]) / sm_count;
-        longest = std::max(longest, 4.0 + kPair[k] * (double)((s.walk[k] + parts[k] - 1) / parts[k]));
+        item[k] = 4.0 + kPair[k] * (double)((s.walk[k] + parts[k] - 1) / parts[k]);
         if (parts[k] > 1) floats += (double)(s.items[k] * parts[k]) * (k == 0 ? 2 : 1) * 128 * 128;
       }
-      const double t = std::max(longest, all + 0.5 * longest) + (floats > 0.0 ? 4.0 + 8.0 * floats / 4e6 : 0.0);
+      const double t = bwd_end(sm_count, s.items[0] * parts[0], item[0], s.items[1] * parts[1], item[1]) +
+                       (floats > 0.0 ? 3.0 + 8.0 * floats / 12e6 : 0.0);
       if (best == 0.0 || t < best) {
         best = t;
         s.parts[0] = a, s.parts[1] = b;

@@ -361,7 +361,7 @@ B200_API int b200_cross_attn_bf16(const b200_attn_view* q, const b200_attn_view*
  * overlap an input or each other.  Workspace:
  * b200_cross_attn_bwd_workspace_bytes, as above: 8 bytes per query row and
  * head, and, where there are fewer 128-row gradient tiles than SMs, up to
- * about 40 MB of fp32 sums.  No reference counterpart
+ * about 60 MB of fp32 sums.  No reference counterpart
  * (the reference has no backward pass).
  */
 B200_API int b200_cross_attn_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
