@@ -46,7 +46,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
 
     A page's scale is the smallest power of two >= 2**-100 that brings its values within 448; it grows while the page
     fills (codes already there are rounded to it) and starts afresh when slot 0 is written.  No page may belong to two
-    sequences of one call.  Lengths or pages out of range leave their sequence unwritten and are raised by
+    sequences of one call or stand twice in one.  Lengths or pages out of range leave their sequence unwritten and are raised by
     check_status()."""
     _binding().kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens, _stream(stream))
 
@@ -60,7 +60,8 @@ def cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_
     q: bf16 [batch, q_len, heads, 128], heads a multiple of kv_heads (query head h reads key/value head
     h // (heads // kv_heads)).  seq_lens: lengths with the new tokens, which are already in the cache; new_lens: how many
     of q's tokens a sequence has (default: q_len).  Query t is at place seq_lens - new_lens + t and attends to the places
-    up to its own.  Rows past new_lens and rows that see nothing are 0.  scale defaults to 128 ** -0.5."""
+    up to its own.  Rows past new_lens and rows that see nothing are 0.  scale defaults to 128 ** -0.5.  out, if given, is shaped like q
+    and does not share q's memory."""
     return _binding().cache_attn(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens, scale, out,
                                  _stream(stream))
 
@@ -74,7 +75,8 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: to
     that keep the last dimension contiguous (a fused projection's views, [batch, heads, tokens, 128] storage).  kv_lens:
     int32 [batch], keys of each entry (default: kv_len); what lies behind them is not used.  An entry without keys gives 0.
     return_lse=True returns (out, lse) with lse float32 [batch, heads, q_len], the natural log of the softmax denominator
-    (-inf without keys), which cross_attn_backward takes.  scale defaults to 128 ** -0.5."""
+    (-inf without keys), which cross_attn_backward takes.  scale defaults to 128 ** -0.5.  out, if given, is shaped like q
+    and shares no memory with the inputs."""
     o, lse = _binding().cross_attn(q, k, v, kv_lens, scale, out, return_lse, _stream(stream))
     return (o, lse) if return_lse else o
 

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kKvWriteThreads) kv_cache_write_kernel(const _
   const int len = p.seq_lens[bat];
   const int fresh = p.new_lens != nullptr ? p.new_lens[bat] : p.new_max;
   const int first = len - fresh;  // place of the first new token
-  if (fresh < 0 || fresh > p.new_max || first < 0 || len > p.max_pages * kPage) {
+  if (len < 0 || fresh < 0 || fresh > p.new_max || first < 0 || len > p.max_pages * kPage) {
     if (threadIdx.x == 0) kv_bad_index(p.status);
     return;
   }

@@ -189,7 +189,7 @@ int check_cache(const b200_kv_cache* c) {
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return B200_ERR_INVALID_ARG;
   if (c->table_stride < c->max_pages) return B200_ERR_INVALID_ARG;
   if (c->num_pages > kLim || c->kv_heads > 65535 || c->num_pages * c->kv_heads > kLim / c->page_size ||
-      c->max_pages > kLim / c->page_size)
+      c->max_pages > (kLim - 128) / c->page_size)
     return B200_ERR_TOO_LARGE;
   return B200_OK;
 }

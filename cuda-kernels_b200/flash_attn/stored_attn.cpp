@@ -152,6 +152,13 @@ void check_like(const char* name, const Tensor& t, const Tensor& q) {
     bad_value(name, " must be ", q.sizes(), " on ", q.device(), ", got ", t.sizes(), " on ", t.device());
 }
 
+// An output tensor of the caller's: like q, but not q itself (warps that share
+// rows of q finish at different times).
+void check_out(const Tensor& out, const Tensor& q) {
+  check_like("out", out, q);
+  if (out.numel() > 0 && out.data_ptr() == q.data_ptr()) bad_value("out may not be q's memory");
+}
+
 // Makes the tensors' device current and picks the stream of a call.
 struct Scope {
   c10::cuda::CUDAGuard device;
@@ -200,7 +207,7 @@ Tensor cache_attn(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
   const int32_t* lens = lens_of("seq_lens", seq_lens, batch, q.device());
   const int32_t* fresh = lens_of("new_lens", new_lens, batch, q.device());
   const float scale = scale_of(scale_in);
-  if (out.has_value()) check_like("out", *out, q);
+  if (out.has_value()) check_out(*out, q);
   const Scope scope(q.device(), stream);
   const Tensor o = out.has_value() ? *out : scope.empty(q.sizes(), torch::kBFloat16);
   const b200_attn_view oo = view_of("out", o);
@@ -237,7 +244,7 @@ std::pair<Tensor, OptTensor> cross_attn(const Tensor& q, const Tensor& k, const 
   const CrossShape s = cross_shape(q, k, v);
   const int32_t* lens = lens_of("kv_lens", kv_lens, s.batch, q.device());
   const float scale = scale_of(scale_in);
-  if (out.has_value()) check_like("out", *out, q);
+  if (out.has_value()) check_out(*out, q);
   const Scope scope(q.device(), stream);
   const Tensor o = out.has_value() ? *out : scope.empty(q.sizes(), torch::kBFloat16);
   const b200_attn_view oo = view_of("out", o);

@@ -297,7 +297,7 @@ typedef struct b200_kv_cache {
  * whose slot 0 is written starts afresh.  Slots behind the new tokens are left
  * as they are.  NaN stays NaN and takes no part in a scale, an infinity
  * counts as bf16's largest value and becomes the largest code.  No page may
- * belong to two sequences that are written in one call.  A sequence whose lengths or pages are out of range is not written
+ * belong to two sequences that are written in one call, or stand twice in one.  A sequence whose lengths or pages are out of range is not written
  * and is reported by b200_gemm_status (B200_ERR_BAD_INDEX).  Asynchronous; no
  * allocation.  No reference counterpart (the reference's attention has no
  * cache).
@@ -317,7 +317,8 @@ B200_API int b200_kv_cache_write(const b200_attn_view* k, const b200_attn_view* 
  * of the cache must be within [2^-100, 2^100].  Lengths and pages out of range
  * are clamped or skipped and reported by b200_gemm_status
  * (B200_ERR_BAD_INDEX); the rows of such a sequence are unspecified.
- * fp32 softmax and accumulation; results do not depend on timing.  The
+ * fp32 softmax and accumulation; results do not depend on timing.  o may not
+ * overlap q.  The
  * workspace (b200_cache_attn_workspace_bytes, 256-byte aligned, no
  * initialisation) may not be shared by calls that can run at the same time.
  * No reference counterpart.

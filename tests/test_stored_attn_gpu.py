@@ -371,6 +371,30 @@ def test_cache_attn_bad_pages_are_reported():
     assert b200_gemm.check_status() == 0
 
 
+@pytest.mark.parametrize("length", [-(1 << 31), -(1 << 31) + 5, -1, (1 << 31) - 1, 65])
+def test_cache_lengths_far_out_of_range(length):
+    """Differences of such lengths wrap around in 32 bits: nothing is written, both calls report, the other sequence is right."""
+    g = torch.Generator().manual_seed(20)
+    cache = _filled(g, [40, 40], 2, 16, most=64)
+    dev = _on(cache)
+    k = _randn(g, 2, 10, 2, 128)
+    lens = torch.tensor([length, 40], dtype=torch.int32)
+    b200_gemm.kv_cache_write(*_on([k, k]), *dev[:5], lens.to(DEV))
+    torch.cuda.synchronize()
+    with pytest.raises(b200_gemm.B200GemmError, match="out of range"):
+        b200_gemm.check_status()
+    want = ref.cache_write(k[1:], k[1:], *cache[:4], cache[4][1:], lens[1:])
+    assert all(_same(a, b) for a, b in zip(dev[:4], want))
+    q = _randn(g, 2, 1, 4, 128)
+    out = b200_gemm.cache_attn(q.to(DEV), *dev[:5], lens.to(DEV))
+    torch.cuda.synchronize()
+    with pytest.raises(b200_gemm.B200GemmError, match="out of range"):
+        b200_gemm.check_status()
+    near = [d.cpu() for d in dev[:4]]
+    value, bound = ref.cache_attn(q[1:], *near, cache[4][1:], lens[1:])
+    _within(out[1:], value, bound)
+
+
 def test_cache_refusals():
     g = torch.Generator().manual_seed(19)
     kc, vc, ks, vs, table, lens = _on(_filled(g, [20], 2, 16))
@@ -406,6 +430,8 @@ def test_cache_refusals():
         attn(q.expand(1, 2, 4, 128), kc, vc, ks, vs, table, lens)
     with pytest.raises(ValueError):
         attn(q, kc, vc, ks, vs, table, lens, out=q[:, :, :2])
+    with pytest.raises(ValueError):
+        attn(q, kc, vc, ks, vs, table, lens, out=q)
     with pytest.raises(ValueError):
         write(k, k[:, :, :1], kc, vc, ks, vs, table, lens)
     with pytest.raises(ValueError):
@@ -569,6 +595,8 @@ def test_cross_refusals():
         f(q[..., :64], k[..., :64], v[..., :64])
     with pytest.raises(ValueError):
         f(q, k, v, out=q[:, :2])
+    with pytest.raises(ValueError):
+        f(q, k, v, out=q)
     assert f(q[:, :0], k, v).shape == (2, 0, 4, 128)
     _ok()
 
