@@ -715,6 +715,39 @@ def test_backward_refusals():
     _ok()
 
 
+def test_backward_workspace_is_checked():
+    """Few gradient tiles: the fp32 sums of their parts are in the workspace, and one byte less is refused."""
+    import ctypes
+
+    from b200_gemm import _lib
+    lib = _lib.load()
+    q, k, v = _on(_cross_inputs(66, 1, 600, 900, 4, 1))
+    out, lse = b200_gemm.cross_attn(q, k, v, return_lse=True)
+    do = torch.ones_like(q)
+    need = ctypes.c_size_t(0)
+    assert lib.b200_cross_attn_bwd_workspace_bytes(1, 600, 900, 4, 1, ctypes.byref(need)) == _lib.B200_OK
+    plain = 256 + 2 * 4 * 4 * 640  # counters, and two floats per padded query row
+    assert need.value > plain
+    ws = torch.empty(need.value, dtype=torch.uint8, device=DEV)
+    grads = [torch.full_like(t, 7.0) for t in (q, k, v)]
+
+    def view(t):
+        return ctypes.byref(_lib.AttnView(t.data_ptr(), *t.stride()[:3]))
+
+    def call(n):
+        return lib.b200_cross_attn_bwd_bf16(view(q), view(k), view(v), view(out), view(do), lse.data_ptr(), None, *map(view, grads),
+                                            1, 600, 900, 4, 1, 128, 128 ** -0.5, ws.data_ptr(), n, None)
+
+    torch.cuda.synchronize()
+    for n in (need.value - 1, plain, plain - 1, 0):
+        assert call(n) == _lib.B200_ERR_INVALID_ARG
+    torch.cuda.synchronize()
+    assert all(bool((t == 7.0).all()) for t in grads)
+    assert call(need.value) == _lib.B200_OK
+    _ok()
+    assert all(torch.equal(a, b) for a, b in zip(grads, b200_gemm.cross_attn_backward(do, q, k, v, out, lse)))
+
+
 def test_training_step_captured_and_on_another_stream():
     """Forward and backward in a captured graph, replayed with new inputs, and on a side stream."""
     g = torch.Generator().manual_seed(64)
